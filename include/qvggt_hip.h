@@ -322,6 +322,60 @@ int qv_attention_fwd(const void* q, const void* k, const void* v, void* out, int
                      int64_t k_token_stride, int64_t v_token_stride, int64_t out_token_stride,
                      float scale, void* stream);
 
+/* -------------------------------------------- streaming: positions and cache
+ * No counterparts in the reference extension: its RoPE ops turn by one axis or
+ * by given angles, and it has no cache that VGGT's blocks could use.
+ */
+
+/*
+ * Rotary positions of several axes on x (T, H, D), fp16 / bf16 / fp32, token and
+ * head strides in elements, dims contiguous; out the same with its own strides,
+ * or x itself.  positions int32 (T, axes), contiguous; sections (host): dims that
+ * turn by each axis, even, together at most D; dims behind them are copied.
+ * QV_ROPE_BLOCK: each axis has its own dims, the halves of which are paired.
+ * QV_ROPE_HALF: the first half of all rotated dims is paired with the second,
+ * section a taking the next sections[a] / 2 pairs.  turns (device, D / 2 float64):
+ * turns per position of each pair (its frequency / 2 pi); pairs of copied dims
+ * take none.  fp32 arithmetic on angles reduced in fp64, one rounding.
+ */
+#define QV_ROPE_BLOCK 0
+#define QV_ROPE_HALF 1
+int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* positions,
+                 const double* turns, const int64_t* sections, int64_t axes, int layout,
+                 int64_t T, int64_t H, int64_t D, int64_t x_token_stride,
+                 int64_t x_head_stride, int64_t out_token_stride, int64_t out_head_stride,
+                 void* stream);
+
+/*
+ * Append to an 8-bit key / value cache: B sequences of `blocks` blocks of 64 tokens,
+ * Hk key heads of D (64 or 128) dims.  k_codes / v_codes: int8, B * Hk * blocks * 64 * D,
+ * in the block layout of qvggt_amd/csrc/kv_cache.h; k_scales / v_scales: fp32 (B, Hk, blocks).
+ * k, v (B, n, Hk, D) fp16 or bf16; k_strides, v_strides (host): their batch, token
+ * and head strides in elements, multiples of 8; dims contiguous.
+ * Sequence b gets its first counts[b] tokens (NULL: n) behind start[b] cached ones
+ * (what it held behind them is dropped, what does not fit is left out), and lens[b] is
+ * set to their number; start may be lens itself.  tickets: B words, 0 at the first
+ * call, kept with the cache.  A block's scale is the smallest number of four
+ * significant bits that is at least amax / 127 over its new tokens, or the one it had
+ * where that is larger; value = code * scale, code = rint(x / scale), ties to even; the
+ * old codes of a block whose scale grows are rounded again.  A NaN or infinity
+ * makes the scale NaN until the block is begun again.
+ */
+int qv_kv8_append(const void* k, const void* v, int dtype, void* k_codes, void* v_codes,
+                  float* k_scales, float* v_scales, const int32_t* start, int32_t* lens,
+                  uint32_t* tickets, const int32_t* counts, int64_t B, int64_t n, int64_t Hk,
+                  int64_t D, int64_t blocks, const int64_t* k_strides,
+                  const int64_t* v_strides, void* stream);
+
+/*
+ * The cached values, code * scale, of tokens first[b] .. first[b] + n - 1 (first
+ * NULL: 0) as k_out, v_out (B, n, Hk, D) fp32, fp16 or bf16; zero behind lens[b].
+ */
+int qv_kv8_values(const void* k_codes, const void* v_codes, const float* k_scales,
+                  const float* v_scales, const int32_t* lens, const int32_t* first,
+                  void* k_out, void* v_out, int dtype, int64_t B, int64_t n, int64_t Hk,
+                  int64_t D, int64_t blocks, void* stream);
+
 /*
  * The launch form that an int8 GEMM (kind 0: weight as stored, 1: packed, 2:
  * int32 output) or qv_f16_gemm (kind 3) picks for M x K -> N, written to

@@ -19,6 +19,8 @@ QV_EPI_NONE = 0
 QV_EPI_BIAS = 1
 QV_EPI_BIAS_GELU = 2
 QV_EPI_GELU = 3
+QV_ROPE_BLOCK = 0
+QV_ROPE_HALF = 1
 
 _vp = C.c_void_p
 _i64 = C.c_int64
@@ -63,6 +65,9 @@ SIGNATURES: dict[str, list] = {
     "qv_adaln_modulate": [_vp, _vp, _vp, _vp, _i64, _i64, _vp],
     "qv_pose_update": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "qv_attention_fwd": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp],
+    "qv_rope_axes": [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32] + [_i64] * 7 + [_vp],
+    "qv_kv8_append": [_vp, _vp, _i32] + [_vp] * 8 + [_i64] * 5 + [_vp] * 3,
+    "qv_kv8_values": [_vp] * 8 + [_i32] + [_i64] * 5 + [_vp],
 }
 _RESTYPES = {"qv_last_error": C.c_char_p, "qv_version": C.c_char_p, "qv_w8a8_packed_bytes": C.c_int64}
 

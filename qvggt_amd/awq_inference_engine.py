@@ -20,6 +20,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -108,6 +110,17 @@ def _check_out(out: torch.Tensor, M: int, N: int, dtype, what: str):
               f"got {tuple(out.shape)}")
     if out.data_ptr() % 16:
         _fail(f"{what}: out must be 16-byte aligned")
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of t may share an address (an expanded tensor, say):
+    not if each dim's stride, in ascending order, passes what the dims below it span."""
+    span = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < span:
+            return True
+        span += st * (n - 1)
+    return False
 
 
 def _check_rope_tables(cos_table: torch.Tensor, sin_table: torch.Tensor, what: str):
@@ -735,6 +748,88 @@ def rope2d_tables(max_position: int, base: float = 100.0, device=None):
     c = torch.from_numpy(np.cos(ang).astype(np.float32))
     s = torch.from_numpy(np.sin(ang).astype(np.float32))
     return (c.to(device), s.to(device)) if device is not None else (c, s)
+
+
+class RopeAxesPlan(NamedTuple):
+    """Which dims of a head turn by which axis, and how fast (``rope_axes_plan``)."""
+    head_dim: int
+    sections: tuple          # dims that turn by each axis
+    layout: str              # "block" or "half"
+    turns: torch.Tensor      # float64 (head_dim / 2,): turns per position of each pair
+
+
+def rope_axes_plan(head_dim: int, sections, base: float = 100.0, layout: str = "block", frequencies=None,
+                   device=None) -> RopeAxesPlan:
+    """Plan of ``rope_axes``: axis a turns ``sections[a]`` dims (even; together at
+    most head_dim, dims behind them are copied).
+
+    layout "block": the dims of an axis are contiguous, their halves paired, pair
+    i of n dims with the frequency base**(-2i/n) (``rope2d``: sections (32, 32)).
+    layout "half": the halves of all R rotated dims are paired, pair j with the
+    frequency base**(-2j/R), and the axes take the pairs in turn.
+    ``frequencies``: R/2 numbers, radians per position, in place of these."""
+    what = "rope_axes_plan"
+    sections = tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 4 or any(n <= 0 or n % 2 for n in sections):
+        _fail(f"{what}: sections must be 1 to 4 positive even numbers of dims, got {sections}")
+    if head_dim <= 0 or head_dim % 2 or head_dim > 1024 or sum(sections) > head_dim:
+        _fail(f"{what}: head_dim {head_dim} must be even, at most 1024 and hold the sections {sections}")
+    if layout not in ("block", "half"):
+        _fail(f"{what}: layout must be 'block' or 'half', got {layout!r}")
+    rot = sum(sections)
+    if frequencies is None:
+        if layout == "half":
+            frequencies = [base ** (-2.0 * j / rot) for j in range(rot // 2)]
+        else:
+            frequencies = [base ** (-2.0 * i / n) for n in sections for i in range(n // 2)]
+    freq = torch.as_tensor(frequencies, dtype=torch.float64).cpu()
+    if tuple(freq.shape) != (rot // 2,) or not bool(torch.isfinite(freq).all()):
+        _fail(f"{what}: frequencies must be {rot // 2} finite numbers")
+    turns = torch.zeros(head_dim // 2, dtype=torch.float64)
+    turns[:rot // 2] = freq / (2.0 * math.pi)
+    return RopeAxesPlan(head_dim, sections, layout, turns.to(device) if device is not None else turns)
+
+
+def rope_axes(x: torch.Tensor, positions: torch.Tensor, plan: RopeAxesPlan, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of several axes on x (T, H, D), fp16 / bf16 / fp32, any
+    token and head strides (e.g. the q and k heads of a fused qkv buffer,
+    ``qkv.view(T, 3 * H, D)[:, :2 * H]``).
+
+    positions int32 (T, axes).  ``out=x`` rotates in place; otherwise out must not
+    overlap x.  Angles are reduced in 64 bits, so far positions lose nothing."""
+    what = "rope_axes"
+    dt = _dtype_any(x, what)
+    if not isinstance(plan, RopeAxesPlan):
+        _fail(f"{what}: plan must come from rope_axes_plan")
+    axes = len(plan.sections)
+    if x.dim() != 3 or x.shape[2] != plan.head_dim:
+        _fail(f"{what}: x must be (T, H, {plan.head_dim}), got {tuple(x.shape)}")
+    T, H, D = x.shape
+    if positions.dtype != torch.int32 or tuple(positions.shape) != (T, axes):
+        _fail(f"{what}: positions must be int32 ({T}, {axes}), got {positions.dtype} {tuple(positions.shape)}")
+    if plan.turns.dtype != torch.float64 or tuple(plan.turns.shape) != (D // 2,) or not plan.turns.is_contiguous():
+        _fail(f"{what}: the plan's turns must be contiguous float64 ({D // 2},)")
+    if out is not None:
+        if out.dtype != x.dtype or out.shape != x.shape or out.stride(2) != 1:
+            _fail(f"{what}: out must be {x.dtype} {tuple(x.shape)} with unit dim stride")
+        if _overlaps_itself(out):
+            _fail(f"{what}: out must not overlap itself")
+        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+            _fail(f"{what}: in place, out must be x")
+    dev = _on_gpu(x, positions, plan.turns, out, what=what)
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    if out is None:
+        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+    if T == 0 or H == 0:
+        return out
+    pos = _contig(positions)
+    sections = (C.c_int64 * axes)(*plan.sections)
+    layout = _lib.QV_ROPE_BLOCK if plan.layout == "block" else _lib.QV_ROPE_HALF
+    with _device(dev):
+        _lib.call("qv_rope_axes", _ptr(x), _ptr(out), dt, _ptr(pos), _ptr(plan.turns), sections, axes, layout, T, H, D,
+                  x.stride(0), x.stride(1), out.stride(0), out.stride(1), _stream(dev))
+    return out
 
 
 # ------------------------------------------------------------- attention

@@ -1,0 +1,257 @@
+// Rotary positions of several axes (time, height, width, ...) for gfx950.
+//
+// A head of D dims is cut into pairs (lo, hi); pair j turns by the angle
+// pos[axis_j] * theta_j: lo' = lo cos - hi sin, hi' = hi cos + lo sin.  The
+// pairs come in chunks of one axis with a fixed distance hi - lo; dims behind
+// the rotated ones form a last chunk that is copied.
+//
+// The angle is a product of an integer position and a frequency that is kept
+// in turns (theta / 2 pi) in 64 bits: t = pos * turns, t - rint(t) is exact, and
+// only the fraction goes to 32 bits.  A 32-bit product would lose pos * 2^-24 of
+// an angle in radians (position 100000: 6e-3); the 64-bit one loses 2^-52 of a
+// turn for each unit of t.
+//
+// A workgroup takes a few tokens with all their heads: its threads load their
+// pieces of x (V dims at lo, V at hi; 16 bytes each where sections and strides
+// allow it), compute one sine and cosine per (token, pair) into LDS while those
+// loads are in flight, and apply them to every head.  Bound by the bytes of x,
+// read once and written once.
+#include "common.h"
+
+namespace qv {
+
+struct RopeAxes {
+  int chunks;
+  int pair0[6];   // first pair of the chunk (the entry behind the last: D / 2)
+  int lo0[5];     // first lo dim
+  int gap[5];     // hi - lo
+  int axis[5];    // column of the positions; -1: copied
+};
+
+constexpr int ROPE_TABLE = 512;   // (token, pair) entries of a workgroup
+constexpr int ROPE_UNITS = 4;     // pieces of x that a thread has in flight
+
+template <int DT, int V>
+struct RopePiece {
+  static constexpr int ES = DT == QV_F32 ? 4 : 2;
+  static constexpr int BYTES = V * ES;
+  static constexpr int WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (BYTES == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (BYTES == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (BYTES == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x, w[1] = u.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* p) const {
+    if constexpr (BYTES == 2) {
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    } else if constexpr (BYTES == 4) {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else if constexpr (BYTES == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (DT == QV_F32) return __builtin_bit_cast(float, w[i]);
+    else return to_f32((uint16_t)(w[i >> 1] >> (16 * (i & 1))), DT == QV_BF16);
+  }
+  __device__ __forceinline__ void set(int i, float v) {
+    if constexpr (DT == QV_F32) {
+      w[i] = __builtin_bit_cast(uint32_t, v);
+    } else {
+      const uint32_t b = from_f32<DT == QV_BF16>(v);
+      if (i & 1) w[i >> 1] |= b << 16;
+      else w[i >> 1] = b;
+    }
+  }
+};
+
+// token tile TB: TB * pairs table entries (at most ROPE_TABLE) and TB * H * groups
+// pieces of x, taken ROPE_UNITS a thread at a time.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void rope_axes_kernel(
+    const uint8_t* x, uint8_t* out, const int32_t* __restrict__ pos, int axes, const double* __restrict__ turns, RopeAxes ra,
+    long T, int H, int pairs, int TB, long x_ts, long x_hs, long o_ts, long o_hs) {   // x and out may be the same
+  __shared__ float2 table[ROPE_TABLE];
+  const int tid = threadIdx.x;
+  const long tok0 = (long)blockIdx.x * TB;
+  const int ntok = (int)(T - tok0 < TB ? T - tok0 : TB);
+  const int groups = pairs / V, per_tok = H * groups, units = ntok * per_tok;
+  constexpr int ES = RopePiece<DT, V>::ES;
+
+  RopePiece<DT, V> lo[ROPE_UNITS], hi[ROPE_UNITS];
+  // where piece u lies: its token in the tile, its byte offsets in x and out, its first pair
+  auto locate = [&](int u, int& tok, int& pair, long& xo, long& oo, int& gap, bool& turn) {
+    tok = u / per_tok;
+    const int rest = u - tok * per_tok;
+    const int head = rest / groups;
+    pair = (rest - head * groups) * V;
+    int lo0 = ra.lo0[0], p0 = 0, ax = ra.axis[0];
+    gap = ra.gap[0];
+#pragma unroll
+    for (int c = 1; c < 5; ++c)
+      if (c < ra.chunks && pair >= ra.pair0[c]) lo0 = ra.lo0[c], p0 = ra.pair0[c], gap = ra.gap[c], ax = ra.axis[c];
+    const int dim = lo0 + pair - p0;
+    turn = ax >= 0;
+    xo = ((tok0 + tok) * x_ts + head * x_hs + dim) * ES;
+    oo = ((tok0 + tok) * o_ts + head * o_hs + dim) * ES;
+  };
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int u = base + 256 * i + tid;
+      if (u < units) {
+        int tok, pair, gap;
+        bool turn;
+        long xo, oo;
+        locate(u, tok, pair, xo, oo, gap, turn);
+        lo[i].load(x + xo);
+        hi[i].load(x + xo + (long)gap * ES);
+      }
+    }
+  };
+  fetch(0);
+  for (int e = tid; e < ntok * pairs; e += 256) {
+    const int tok = e / pairs, pair = e - tok * pairs;
+    int ax = ra.axis[0];
+#pragma unroll
+    for (int c = 1; c < 5; ++c)
+      if (c < ra.chunks && pair >= ra.pair0[c]) ax = ra.axis[c];
+    float s = 0.f, c = 1.f;
+    if (ax >= 0) {
+      const double t = (double)pos[(tok0 + tok) * axes + ax] * turns[pair];
+      sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    }
+    table[e] = make_float2(c, s);
+  }
+  __syncthreads();
+  for (int base = 0; base < units; base += 256 * ROPE_UNITS) {
+    if (base) fetch(base);
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int u = base + 256 * i + tid;
+      if (u < units) {
+        int tok, pair, gap;
+        bool turn;
+        long xo, oo;
+        locate(u, tok, pair, xo, oo, gap, turn);
+        if (turn) {
+          RopePiece<DT, V> a, b;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float2 cs = table[tok * pairs + pair + e];
+            const float l = lo[i].get(e), h = hi[i].get(e);
+            a.set(e, __builtin_fmaf(l, cs.x, -(h * cs.y)));
+            b.set(e, __builtin_fmaf(h, cs.x, l * cs.y));
+          }
+          a.store(out + oo);
+          b.store(out + oo + (long)gap * ES);
+        } else {
+          lo[i].store(out + oo);
+          hi[i].store(out + oo + (long)gap * ES);
+        }
+      }
+    }
+  }
+}
+
+template <int DT>
+static void rope_axes_launch(int vec, unsigned grid, hipStream_t st, const void* x, void* out, const int32_t* pos, int axes,
+                             const double* turns, const RopeAxes& ra, long T, int H, int pairs, int TB, long x_ts,
+                             long x_hs, long o_ts, long o_hs) {
+#define QV_ROPE(V)                                                                                                   \
+  hipLaunchKernelGGL((rope_axes_kernel<DT, V>), dim3(grid), dim3(256), 0, st, (const uint8_t*)x, (uint8_t*)out, pos, \
+                     axes, turns, ra, T, H, pairs, TB, x_ts, x_hs, o_ts, o_hs)
+  if (vec == 8) QV_ROPE(8);
+  else if (vec == 4) QV_ROPE(4);
+  else if (vec == 2) QV_ROPE(2);
+  else QV_ROPE(1);
+#undef QV_ROPE
+}
+
+}  // namespace qv
+
+extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* positions, const double* turns,
+                            const int64_t* sections, int64_t axes, int layout, int64_t T, int64_t H, int64_t D,
+                            int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride,
+                            int64_t out_head_stride, void* stream) {
+  QV_CHECK_ARG(dtype == QV_F16 || dtype == QV_BF16 || dtype == QV_F32, "bad dtype %d", dtype);
+  QV_CHECK_ARG(axes >= 1 && axes <= 4, "1 to 4 axes are supported (got %lld)", (long long)axes);
+  QV_CHECK_ARG(layout == QV_ROPE_BLOCK || layout == QV_ROPE_HALF, "bad layout %d", layout);
+  QV_CHECK_ARG(T >= 0 && H > 0 && D > 0 && D % 2 == 0 && D <= 1024 && H <= 65536, "bad shape T=%lld H=%lld D=%lld",
+               (long long)T, (long long)H, (long long)D);
+  QV_CHECK_ARG(sections, "null sections");
+  qv::RopeAxes ra = {};
+  int64_t rot = 0;
+  for (int a = 0; a < axes; ++a) {
+    QV_CHECK_ARG(sections[a] > 0 && sections[a] % 2 == 0 && sections[a] <= D,
+                 "section %d must be a positive even number of dims (got %lld)", a, (long long)sections[a]);
+    rot += sections[a];
+  }
+  QV_CHECK_ARG(rot <= D, "sections hold %lld dims of %lld", (long long)rot, (long long)D);
+  if (T == 0) return QV_OK;
+  QV_CHECK_ARG(x && out && positions && turns, "null pointer argument");
+  int64_t at = 0;
+  for (int a = 0; a < axes; ++a) {
+    ra.pair0[a] = (int)(at / 2);
+    ra.lo0[a] = (int)(layout == QV_ROPE_BLOCK ? at : at / 2);
+    ra.gap[a] = (int)(layout == QV_ROPE_BLOCK ? sections[a] / 2 : rot / 2);
+    ra.axis[a] = a;
+    at += sections[a];
+  }
+  ra.chunks = (int)axes;
+  if (rot < D) {
+    ra.pair0[axes] = (int)(rot / 2);
+    ra.lo0[axes] = (int)rot;
+    ra.gap[axes] = (int)(D - rot) / 2;
+    ra.axis[axes] = -1;
+    ra.chunks = (int)axes + 1;
+  }
+  ra.pair0[ra.chunks] = (int)(D / 2);
+  // the widest piece that starts on its own multiple everywhere: inside the
+  // chunks, and at every head and token of x and out
+  const int es = dtype == QV_F32 ? 4 : 2;
+  int vec = 8;
+  auto fits = [&](int64_t v) { return v % vec == 0; };
+  for (;; vec /= 2) {
+    const int align = vec * es < 16 ? vec * es : 16;
+    bool ok = fits(x_token_stride) && fits(x_head_stride) && fits(out_token_stride) && fits(out_head_stride) &&
+              fits(D / 2) && (uintptr_t)x % align == 0 && (uintptr_t)out % align == 0;
+    for (int c = 0; c < ra.chunks; ++c) ok = ok && fits(ra.pair0[c]) && fits(ra.lo0[c]) && fits(ra.gap[c]);
+    if (ok || vec == 1) break;
+  }
+  QV_CHECK_ARG((uintptr_t)x % es == 0 && (uintptr_t)out % es == 0, "x and out must be aligned to their type");
+  const int pairs = (int)(D / 2);
+  const int64_t per_tok = H * (pairs / vec);
+  // tokens of a workgroup: one piece round (1024 pieces), at most the table, and
+  // enough workgroups to fill the chip
+  int64_t tb = 256 * qv::ROPE_UNITS / per_tok;
+  if (tb > qv::ROPE_TABLE / pairs) tb = qv::ROPE_TABLE / pairs;
+  if (tb > T / 1024) tb = T / 1024;
+  if (tb < 1) tb = 1;
+  const int64_t grid = (T + tb - 1) / tb;
+  QV_CHECK_ARG(grid <= INT32_MAX && per_tok * tb <= INT32_MAX / 2, "too many tokens or heads");
+#define QV_ARGS                                                                                                       \
+  vec, (unsigned)grid, (hipStream_t)stream, x, out, positions, (int)axes, turns, ra, (long)T, (int)H, pairs, (int)tb, \
+      (long)x_token_stride, (long)x_head_stride, (long)out_token_stride, (long)out_head_stride
+  if (dtype == QV_F16) qv::rope_axes_launch<QV_F16>(QV_ARGS);
+  else if (dtype == QV_BF16) qv::rope_axes_launch<QV_BF16>(QV_ARGS);
+  else qv::rope_axes_launch<QV_F32>(QV_ARGS);
+#undef QV_ARGS
+  return qv::check_launch("rope_axes");
+}

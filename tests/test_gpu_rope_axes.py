@@ -1,0 +1,107 @@
+"""rope_axes against the float64 oracle.
+
+Bound: the fraction of a turn is rounded to fp32 (half a turn * 2^-24 * 2 pi =
+3.2 * 2^-24 radians), sincospif is within 2 ulp (2^-23 at 1), the product and the
+fused multiply-add round once each: under 8 * 2^-24 of |lo| + |hi| together; then
+half a step of the output's type.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import streaming as O
+
+pytestmark = pytest.mark.gpu
+
+STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 0.0, torch.float32: 0.0}
+
+
+def _check(got, x, pos, pairs):
+    x = x.double().cpu().numpy()
+    ref = O.rope_axes(x, pos.cpu().numpy(), pairs)
+    size = np.zeros(x.shape)
+    for lo, hi, _, _ in pairs:
+        size[..., lo] = size[..., hi] = np.abs(x[..., lo]) + np.abs(x[..., hi])
+    err = np.abs(got.double().cpu().numpy() - ref)
+    step = STEP[got.dtype]
+    assert (err <= np.abs(ref) * step + size * 8 * 2.0 ** -24 * (1 + step) + TINY[got.dtype]).all(), err.max()
+
+
+@pytest.mark.parametrize("D,sections,layout", [
+    (64, (32, 32), "block"), (64, (16, 24, 24), "block"), (64, (10, 26, 28), "block"), (64, (16, 8), "half"),
+    (128, (32, 48, 48), "half"), (128, (22, 50, 56), "half"), (128, (64, 32), "block"), (16, (2, 2, 4, 8), "block"),
+    (1024, (512, 512), "half"), (6, (2, 4), "half")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,H", [(1, 1), (3, 5), (200, 3), (2500, 2)])
+def test_rope_axes(gpu, D, sections, layout, dtype, T, H):
+    """Every piece width (16 bytes down to one element), copied dims, one to four axes, far and negative positions."""
+    from qvggt_amd import awq_inference_engine as E
+    g = torch.Generator(device=gpu).manual_seed(D + T)
+    x = torch.randn(T, H, D, generator=g, device=gpu).to(dtype)
+    pos = torch.randint(-100, 2000000, (T, len(sections)), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(D, sections, layout=layout, device=gpu)
+    out = E.rope_axes(x, pos, plan)
+    _check(out, x, pos, O.rope_pairs(sections, layout))
+    rot = sum(sections)
+    assert torch.equal(out[..., rot:], x[..., rot:])
+
+
+def test_rope_axes_views_and_in_place(gpu):
+    """The q and k heads inside a fused qkv buffer, rotated in place: the v heads stay, the bits are those of a copy."""
+    from qvggt_amd import awq_inference_engine as E
+    T, H, D = 333, 4, 64
+    g = torch.Generator(device=gpu).manual_seed(0)
+    qkv = torch.randn(T, 3 * H, D, generator=g, device=gpu).half()
+    pos = torch.randint(0, 40, (T, 3), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(D, (16, 24, 24), device=gpu)
+    want = E.rope_axes(qkv[:, :2 * H].contiguous(), pos, plan)
+    keep = qkv[:, 2 * H:].clone()
+    got = E.rope_axes(qkv[:, :2 * H], pos, plan, out=qkv[:, :2 * H])
+    assert torch.equal(got, want) and torch.equal(qkv[:, 2 * H:], keep)
+    # odd strides and addresses: narrower pieces, the same bits
+    wide = torch.randn(T * (2 * H * (D + 3)) + 1, generator=g, device=gpu).half()
+    odd = wide[1:].view(T, 2 * H, D + 3)[..., :D]
+    src = odd.clone()
+    out = E.rope_axes(odd, pos, plan)
+    assert torch.equal(out, E.rope_axes(src.contiguous(), pos, plan))
+    # heads before tokens; dims not contiguous (copied)
+    perm = src.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(E.rope_axes(perm, pos, plan), out)
+    assert torch.equal(E.rope_axes(src.transpose(1, 2).contiguous().transpose(1, 2), pos, plan), out)
+
+
+def test_rope_axes_other_stream_graph_and_empty(gpu):
+    from qvggt_amd import awq_inference_engine as E
+    g = torch.Generator(device=gpu).manual_seed(5)
+    x = torch.randn(100, 8, 128, generator=g, device=gpu).bfloat16()
+    pos = torch.randint(0, 4000, (100, 3), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(128, (32, 48, 48), layout="half", device=gpu)
+    want = E.rope_axes(x, pos, plan)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        other = E.rope_axes(x, pos, plan)
+    torch.cuda.synchronize()
+    assert torch.equal(other, want)
+    out = torch.empty_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.rope_axes(x, pos, plan, out=out)
+    for i in range(3):
+        pos.add_(7)
+        want = E.rope_axes(x, pos, plan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert E.rope_axes(x[:0], pos[:0], plan).shape == (0, 8, 128)
+
+
+def test_rope_axes_non_finite_stays_in_its_pair(gpu):
+    from qvggt_amd import awq_inference_engine as E
+    x = torch.ones(4, 2, 64, device=gpu).half()
+    x[1, 0, 3], x[2, 1, 40] = float("nan"), float("inf")
+    pos = torch.full((4, 1), 5, dtype=torch.int32, device=gpu)
+    out = E.rope_axes(x, pos, E.rope_axes_plan(64, (32,), device=gpu))
+    bad = ~torch.isfinite(out)
+    assert bad.nonzero().tolist() == [[1, 0, 3], [1, 0, 19], [2, 1, 40]]

@@ -1,0 +1,137 @@
+"""Pins of oracle/streaming.py, and the host side of the streaming ops: plans, cache layout, refusals."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as OA
+from oracle import rope as OR
+from oracle import streaming as O
+from qvggt_amd import awq_inference_engine as E
+from qvggt_amd.kv_cache import Int8KVCache
+
+
+# ------------------------------------------------------------------- oracle
+def test_rope_axes_quarter_turn_and_copy():
+    """One pair of one axis at 2 pi / 4 radians a position: position 1 maps (a, b) to (-b, a)."""
+    x = np.array([[[3.0, 5.0, 7.0, 9.0]]] * 2)
+    y = O.rope_axes(x, [[0], [1]], [(0, 1, 0, np.pi / 2)])
+    assert np.array_equal(y[0], x[0])
+    np.testing.assert_allclose(y[1, 0], [-5, 3, 7, 9], atol=1e-14)
+
+
+def test_rope_axes_block_layout_is_rope2d():
+    T, H = 50, 3
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((T, H, 64)).astype(np.float16)
+    pos = rng.integers(0, 38, (T, 2)).astype(np.int32)
+    want = np.asarray(OR.rope2d(x, pos, *OR.rope2d_tables(38)), np.float64)
+    np.testing.assert_allclose(O.rope_axes(x, pos, O.rope_pairs((32, 32), "block")), want, atol=4e-3)   # want is fp16
+
+
+def test_rope_pairs_half_layout():
+    p = O.rope_pairs((4, 2), "half", 10.0)
+    assert [t[:3] for t in p] == [(0, 3, 0), (1, 4, 0), (2, 5, 1)]
+    assert [t[3] for t in p] == [1.0, 10.0 ** (-2 / 6), 10.0 ** (-4 / 6)]
+
+
+@pytest.mark.parametrize("amax,scale", [(127.0, 1.0), (126.0, 1.0), (127.1, 1.125), (1.0, 9 / 1024),
+                                        (65504.0, 576.0), (0.0, 0.0), (2.0 ** -24, 9 * 2.0 ** -34), (1e-37, 2.0 ** -120)])
+def test_scale_by_hand(amax, scale):
+    """127 -> 1; 127.1 -> the next number of four bits, 1.125; 1/127 = 8.06 / 1024 ->
+    9 / 1024; 65504 / 127 = 515.8 -> 1.125 * 512."""
+    assert O.scale_of(amax) == scale
+
+
+def test_cache_codes_by_hand():
+    c = O.Cache(128, 1, 2)
+    c.append(np.array([[[127.0, -0.5]], [[1.5, 2.5]]]))            # scale 1, ties to even
+    assert c.scales[0, 0] == 1 and c.codes[:2, 0].tolist() == [[127, 0], [2, 2]]
+    c.append(np.array([[[250.0, -4.0]]]))                          # 250 / 127 = 1.97 -> 2: codes halve
+    assert c.scales[0, 0] == 2 and c.codes[:3, 0].tolist() == [[64, 0], [1, 1], [125, -2]]
+    c.append(np.array([[[4.0, 0.0]]]))                             # the scale stays
+    assert c.scales[0, 0] == 2 and c.codes[3, 0].tolist() == [2, 0] and c.len == 4
+    c.append(np.zeros((0, 1, 2)), start=3)
+    assert c.len == 3 and c.values().tolist()[2] == [[250, -4]]
+
+
+def test_attention_agrees_with_the_square_one():
+    rng = np.random.default_rng(1)
+    q, k, v = (rng.standard_normal((20, 2, 64)) for _ in range(3))
+    np.testing.assert_allclose(O.attention(q, k, v, 0.125), OA.attention_ref(q, k, v, 1, 20), atol=1e-12)
+    keep = np.zeros(20, bool)
+    keep[[3, 7]] = True
+    np.testing.assert_allclose(O.attention(q, k, v, 0.125, keep),
+                               O.attention(q, k[[3, 7]], v[[3, 7]], 0.125), atol=1e-12)
+    assert not O.attention(q, k, v, 0.125, np.zeros(20, bool)).any()
+    v[4] = np.nan                                                  # not kept, not read
+    assert np.isfinite(O.attention(q, k, v, 0.125, keep)).all()
+    shared = O.attention(np.repeat(q, 2, 1), k, v[:, :], 0.125, keep)
+    np.testing.assert_array_equal(shared[:, 0], O.attention(q, k, v, 0.125, keep)[:, 0])
+
+
+# ------------------------------------------------------------------ host side
+def test_rope_axes_plan():
+    p = E.rope_axes_plan(64, (16, 24, 20), base=50.0)
+    want = [t[3] / (2 * np.pi) for t in O.rope_pairs((16, 24, 20), "block", 50.0)]
+    assert p.turns[:30].tolist() == pytest.approx(want, rel=1e-15) and p.turns[30:].tolist() == [0, 0]
+    f = E.rope_axes_plan(64, (32,), frequencies=np.arange(16.0), layout="half")
+    assert f.turns[:16].tolist() == pytest.approx((np.arange(16) / (2 * np.pi)).tolist(), rel=1e-15)
+    for bad in (dict(head_dim=64, sections=(15, 3)), dict(head_dim=64, sections=(64, 2)), dict(head_dim=64, sections=()),
+                dict(head_dim=64, sections=(2,) * 5), dict(head_dim=63, sections=(2,)), dict(head_dim=64, sections=(0, 2)),
+                dict(head_dim=64, sections=(4,), layout="x"), dict(head_dim=64, sections=(4,), frequencies=[1.0]),
+                dict(head_dim=64, sections=(4,), frequencies=[1.0, float("nan")])):
+        with pytest.raises(RuntimeError, match="rope_axes_plan"):
+            E.rope_axes_plan(**bad)
+
+
+def test_rope_axes_refusals():
+    plan = E.rope_axes_plan(64, (32, 32))
+    x = torch.zeros(5, 3, 64, dtype=torch.float16)
+    pos = torch.zeros(5, 2, dtype=torch.int32)
+    for args, msg in (((x[..., :32], pos, plan), "x must be"), ((x[0], pos, plan), "x must be"),
+                      ((x.double(), pos, plan), "unsupported dtype"), ((x, pos.long(), plan), "positions must be"),
+                      ((x, pos[:4], plan), "positions must be"), ((x, pos[:, :1], plan), "positions must be"),
+                      ((x, pos, plan.turns), "plan must come"), ((x, pos, plan, x.float()), "out must be"),
+                      ((x, pos, plan, torch.zeros(5, 1, 64).half().expand(5, 3, 64)), "overlap itself"),
+                      ((x, pos, plan, torch.zeros(5, 3, 128).half()[..., ::2]), "unit dim stride"),
+                      ((x[:, :2], pos, plan, x.view(-1)[:640].view(5, 2, 64)), "in place"),
+                      ((x, pos, plan._replace(turns=plan.turns.float())), "turns"),
+                      ((x, pos, plan), "GPU only")):
+        with pytest.raises(RuntimeError, match=msg):
+            E.rope_axes(*args)
+
+
+def test_cache_refusals():
+    for bad in (dict(batch=0, kv_heads=1, head_dim=64, capacity=1), dict(batch=1, kv_heads=0, head_dim=64, capacity=1),
+                dict(batch=1, kv_heads=1, head_dim=96, capacity=1), dict(batch=1, kv_heads=1, head_dim=64, capacity=0)):
+        with pytest.raises(RuntimeError, match="Int8KVCache"):
+            Int8KVCache(**bad, device="cpu")
+    c = Int8KVCache(2, 3, 64, 100, device="cpu")
+    assert c.capacity == 128 and c.blocks == 2
+    k = torch.zeros(2, 5, 3, 64, dtype=torch.float16)
+    one = torch.zeros(2, dtype=torch.int32)
+    for args, kw, msg in (((k, k[:, :4]), {}, "v must be"), ((k.float(), k), {}, "data type"), ((k, k.bfloat16()), {}, "v must be"),
+                          ((k[:1], k[:1]), {}, "k must be"), ((k[..., :32], k), {}, "k must be"),
+                          ((torch.zeros(2, 129, 3, 64).half(),) * 2, {}, "do not fit"),
+                          ((k, k), dict(counts=one.long()), "counts must be"), ((k, k), dict(start=one[:1]), "start must be"),
+                          ((k, k), dict(start=torch.zeros(2, 2, dtype=torch.int32)[:, 0]), "contiguous"),
+                          ((k, k), {}, "GPU only")):
+        with pytest.raises(RuntimeError, match=msg):
+            c.append(*args, **kw)
+    for kw, msg in ((dict(n=-1), "number of tokens"), (dict(dtype=torch.int8), "dtype"), (dict(first=one.float()), "first must"),
+                    ({}, "GPU only")):
+        with pytest.raises(RuntimeError, match=msg):
+            c.values(**kw)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_cache_block_order_is_a_permutation(D):
+    key, val = Int8KVCache(1, 1, D, 64, device="cpu")._order()
+    for o in (key, val):
+        assert o.shape == (64, D) and torch.equal(o.reshape(-1).sort()[0], torch.arange(64 * D))
+    # a lane's unit: 16 dims of one token; the 16 tokens of one dim that its registers meet
+    assert (key.view(64, D // 16, 16).diff(dim=2) == 1).all()
+    toks = torch.empty(64 * D, dtype=torch.long)
+    toks[val.reshape(-1)] = torch.arange(64 * D) // D
+    assert toks[:16].tolist() == [0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27]
+    assert toks[32 * 16:33 * 16].tolist() == [4, 5, 6, 7, 12, 13, 14, 15, 20, 21, 22, 23, 28, 29, 30, 31]
