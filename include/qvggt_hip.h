@@ -377,6 +377,43 @@ int qv_kv8_values(const void* k_codes, const void* v_codes, const float* k_scale
                   int64_t D, int64_t blocks, void* stream);
 
 /*
+ * Attention of queries over keys of another length: q (B, Lq, H, D) and k, v (B, Lk,
+ * Hk, D) fp16 or bf16, D 64 or 128, H a multiple of Hk (query head h reads key head
+ * h / (H / Hk)); out = softmax(q k^T scale) v, fp32 softmax and sums.  The four stride
+ * arrays (host) hold batch, token and head strides in elements: multiples of 8 (out:
+ * of 4), k and v token strides D to 2^24; dims contiguous.  lens (int32, B; NULL: Lk): keys
+ * of each sequence.  mask (B rows of Lk bytes, mask_stride apart; NULL: none): keys
+ * with a 0 are left out.  What is left out may hold anything; a query that no key is
+ * left for gives 0.
+ * workspace: 16-byte aligned, qv_attention_kv_workspace bytes let the key range be
+ * split over workgroups where there are few queries; with less (or NULL) it is split
+ * less or not at all.  Contents need not be kept or cleared.
+ */
+int qv_attention_cross(const void* q, const void* k, const void* v, void* out, int dtype,
+                       const int32_t* lens, const uint8_t* mask, int64_t mask_stride,
+                       int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hk, int64_t D,
+                       const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, const int64_t* out_strides, float scale,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same over the cache of qv_kv8_append, keys 0 .. lens[b] - 1.  counts (B; NULL: Lq):
+ * queries of each sequence; the rows of out behind them are left as they were.
+ * causal: the queries are the last counts[b] tokens, each sees the keys up to its
+ * own.  keys: tokens that a sequence may hold, for the split only.
+ */
+int qv_kv8_attention(const void* q, void* out, int dtype, const void* k_codes,
+                     const void* v_codes, const float* k_scales, const float* v_scales,
+                     const int32_t* lens, const int32_t* counts, int causal, int64_t B,
+                     int64_t Lq, int64_t H, int64_t Hk, int64_t D, int64_t blocks,
+                     int64_t keys, const int64_t* q_strides, const int64_t* out_strides,
+                     float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of the two (cached 0: cross, 1: cache) for keys tokens; 0: none. */
+int64_t qv_attention_kv_workspace(int cached, int64_t B, int64_t Lq, int64_t H, int64_t Hk,
+                                  int64_t D, int64_t keys);
+
+/*
  * The launch form that an int8 GEMM (kind 0: weight as stored, 1: packed, 2:
  * int32 output) or qv_f16_gemm (kind 3) picks for M x K -> N, written to
  * plan[2]: plan[0] = rows of a tile (32, 64, 96 or 128), plan[1] = 2 if K is

@@ -67,9 +67,13 @@ SIGNATURES: dict[str, list] = {
     "qv_attention_fwd": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp],
     "qv_rope_axes": [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32] + [_i64] * 7 + [_vp],
     "qv_kv8_append": [_vp, _vp, _i32] + [_vp] * 8 + [_i64] * 5 + [_vp] * 3,
+    "qv_attention_cross": [_vp] * 4 + [_i32, _vp, _vp] + [_i64] * 7 + [_vp] * 4 + [_f32, _vp, _i64, _vp],
+    "qv_kv8_attention": [_vp, _vp, _i32] + [_vp] * 6 + [_i32] + [_i64] * 7 + [_vp, _vp, _f32, _vp, _i64, _vp],
+    "qv_attention_kv_workspace": [_i32] + [_i64] * 6,
     "qv_kv8_values": [_vp] * 8 + [_i32] + [_i64] * 5 + [_vp],
 }
-_RESTYPES = {"qv_last_error": C.c_char_p, "qv_version": C.c_char_p, "qv_w8a8_packed_bytes": C.c_int64}
+_RESTYPES = {"qv_last_error": C.c_char_p, "qv_version": C.c_char_p, "qv_w8a8_packed_bytes": C.c_int64,
+             "qv_attention_kv_workspace": C.c_int64}
 
 _lock = threading.Lock()
 _lib = None

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple
 
@@ -861,6 +862,89 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_len: int, s
     with _device(dev):
         _lib.call("qv_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), T // seq_len, seq_len, H, 64,
                   q.stride(0), k.stride(0), v.stride(0), out.stride(0), scale, _stream(dev))
+    return out
+
+
+def _kv_rows(t: torch.Tensor) -> torch.Tensor:
+    """t (B, n, H, D), or a copy, as the attention and cache kernels read it: dims
+    contiguous, rows on 16 bytes, tokens not overlapping."""
+    sb, st, sh, sd = t.stride()
+    B, n, H, D = t.shape
+    if (sd == 1 and t.data_ptr() % 16 == 0 and (sb % 8 == 0 or B == 1) and (sh % 8 == 0 or H == 1)
+            and (n == 1 or (st % 8 == 0 and D <= st <= 1 << 24))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _kv_strides(t: torch.Tensor):
+    """Batch, token and head strides; 0 for a dim of one."""
+    return (C.c_int64 * 3)(*(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv_workspace_bytes(cached: int, *shape: int) -> int:
+    return _lib.load().qv_attention_kv_workspace(cached, *shape)
+
+
+def _kv_query(q: torch.Tensor, kv_heads: int, out: torch.Tensor | None, scale: float | None, what: str):
+    """Checks that cross and cached attention share; returns (dtype code, scale)."""
+    dt = _dtype_code(q, what)
+    if q.dim() != 4 or q.shape[3] not in (64, 128):
+        _fail(f"{what}: q must be (B, n, heads, 64 or 128), got {tuple(q.shape)}")
+    if kv_heads < 1 or q.shape[2] < 1 or q.shape[2] % kv_heads:
+        _fail(f"{what}: {q.shape[2]} query heads are not a multiple of {kv_heads} key heads")
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        _fail(f"{what}: scale must be a positive number, got {scale}")
+    if out is not None:
+        if out.dtype != q.dtype or out.shape != q.shape or out.stride(3) != 1 or _overlaps_itself(out):
+            _fail(f"{what}: out must be {q.dtype} {tuple(q.shape)} with unit dim stride")
+        if out.data_ptr() % 8 or any(s % 4 for s, n in zip(out.stride()[:3], out.shape[:3]) if n > 1):
+            _fail(f"{what}: out must be 8-byte aligned, its strides multiples of 4 elements")
+    return dt, scale
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
+                    kv_lens: torch.Tensor | None = None, key_mask: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of queries over an encoder's states of another length.
+
+    q (B, Lq, H, D), k and v (B, Lk, Hk, D), all fp16 or all bf16, D 64 or 128, H a
+    multiple of Hk (query head h reads key head h // (H / Hk)), any strides with
+    contiguous dims (others are copied); scale defaults to D**-0.5.  kv_lens
+    int32 (B,): keys of each sequence (drawn into 0..Lk).  key_mask bool (B, Lk):
+    True where a key is attended to.  What they leave out may hold anything,
+    NaN included; a query with no key left gives zeros.  ``out`` must not
+    overlap the inputs."""
+    what = "cross_attention"
+    if k.dim() != 4 or v.shape != k.shape:
+        _fail(f"{what}: k and v must be (B, Lk, kv_heads, D) alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+    dt, scale = _kv_query(q, k.shape[2], out, scale, what)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        _fail(f"{what}: k and v must be {q.dtype}, got {k.dtype} and {v.dtype}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D:
+        _fail(f"{what}: k must be ({B}, Lk, kv_heads, {D}), got {tuple(k.shape)}")
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,) or not kv_lens.is_contiguous()):
+        _fail(f"{what}: kv_lens must be contiguous int32 ({B},), got {kv_lens.dtype} {tuple(kv_lens.shape)}")
+    if key_mask is not None and (key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, Lk)):
+        _fail(f"{what}: key_mask must be bool ({B}, {Lk}), got {key_mask.dtype} {tuple(key_mask.shape)}")
+    dev = _on_gpu(q, k, v, kv_lens, key_mask, out, what=what)
+    q, k, v = _kv_rows(q), _kv_rows(k), _kv_rows(v)
+    mask_stride = 0
+    if key_mask is not None:
+        if Lk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        mask_stride = key_mask.stride(0)
+    if out is None:
+        out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    ws_bytes = _kv_workspace_bytes(0, B, Lq, H, Hk, D, Lk)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _device(dev):
+        _lib.call("qv_attention_cross", _ptr(q), _ptr(k), _ptr(v), _ptr(out), dt, _ptr(kv_lens), _ptr(key_mask), mask_stride,
+                  B, Lq, Lk, H, Hk, D, _kv_strides(q), _kv_strides(k), _kv_strides(v), _kv_strides(out), scale, _ptr(ws),
+                  ws_bytes, _stream(dev))
     return out
 
 

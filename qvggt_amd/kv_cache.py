@@ -8,21 +8,13 @@ the reference extension's decode attention keeps a 16-bit cache of its own layou
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .awq_inference_engine import _contig, _device, _dtype_code, _fail, _on_gpu, _ptr, _stream
+from .awq_inference_engine import (_device, _dtype_code, _fail, _kv_query, _kv_rows, _kv_strides, _kv_workspace_bytes,
+                                   _on_gpu, _ptr, _stream)
 
 BLOCK = 64   # tokens of a block
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t (B, n, H, D), or a copy, as the kernels read it: dims contiguous, 16-byte rows."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3]):
-        return t
-    return t.contiguous()
 
 
 class Int8KVCache:
@@ -59,11 +51,13 @@ class Int8KVCache:
         self.v_scales = torch.zeros(shape[:3], dtype=torch.float32, **kw)
         self.lens = torch.zeros(batch, dtype=torch.int32, **kw)
         self._tickets = torch.zeros(batch, dtype=torch.int32, **kw)
+        self._bound = 0
 
     # ------------------------------------------------------------- contents
     def reset(self) -> None:
         """Forget all tokens."""
         self.lens.zero_()
+        self._bound = 0
 
     def _per_sequence(self, t: torch.Tensor | None, what: str, name: str) -> None:
         if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (self.batch,) or not t.is_contiguous()):
@@ -90,13 +84,14 @@ class Int8KVCache:
         self._per_sequence(counts, what, "counts")
         self._per_sequence(start, what, "start")
         dev = _on_gpu(k, v, counts, start, self.lens, what=what)
-        k, v = _rows(k), _rows(v)
-        ks, vs = (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3])
+        k, v = _kv_rows(k), _kv_rows(v)
         with _device(dev):
             _lib.call("qv_kv8_append", _ptr(k), _ptr(v), dt, _ptr(self.k_codes), _ptr(self.v_codes), _ptr(self.k_scales),
                       _ptr(self.v_scales), _ptr(self.lens if start is None else start), _ptr(self.lens),
-                      _ptr(self._tickets), _ptr(counts), self.batch, n, self.kv_heads, self.head_dim, self.blocks, ks, vs,
-                      _stream(dev))
+                      _ptr(self._tickets), _ptr(counts), self.batch, n, self.kv_heads, self.head_dim, self.blocks,
+                      _kv_strides(k), _kv_strides(v), _stream(dev))
+        # how long a sequence may be by now: a hint for the attention's split of the keys
+        self._bound = min(self.capacity, self._bound + n)
 
     def values(self, n: int | None = None, first: torch.Tensor | None = None, dtype: torch.dtype = torch.float32):
         """The cached (keys, values) of n tokens (default: the capacity) of each sequence
@@ -118,6 +113,35 @@ class Int8KVCache:
                       _ptr(self.lens), _ptr(first), _ptr(k), _ptr(v), dt, self.batch, n, self.kv_heads, self.head_dim,
                       self.blocks, _stream(dev))
         return k, v
+
+    # ------------------------------------------------------------ attention
+    def attention(self, q: torch.Tensor, scale: float | None = None, causal: bool = False,
+                  counts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of q (B, n, heads, head_dim), fp16 or bf16, over the cached tokens of
+        each sequence; heads a multiple of kv_heads, scale head_dim**-0.5 by default.
+
+        causal: the queries are the sequence's last n tokens, each sees the tokens
+        up to its own.  counts int32 (B,): how many of the n queries each sequence
+        has; the rows of ``out`` behind them are left as they were (zero in a new
+        out).  A query that sees no token gives zeros.  Returns (B, n, heads, head_dim)."""
+        what = "Int8KVCache.attention"
+        dt, scale = _kv_query(q, self.kv_heads, out, scale, what)
+        B, n, H, D = q.shape
+        if B != self.batch or D != self.head_dim:
+            _fail(f"{what}: q must be ({self.batch}, n, heads, {self.head_dim}), got {tuple(q.shape)}")
+        self._per_sequence(counts, what, "counts")
+        dev = _on_gpu(q, counts, out, self.lens, what=what)
+        q = _kv_rows(q)
+        if out is None:
+            new = torch.empty if counts is None else torch.zeros
+            out = new((B, n, H, D), dtype=q.dtype, device=q.device)
+        ws_bytes = _kv_workspace_bytes(1, B, n, H, self.kv_heads, D, self._bound)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        with _device(dev):
+            _lib.call("qv_kv8_attention", _ptr(q), _ptr(out), dt, _ptr(self.k_codes), _ptr(self.v_codes), _ptr(self.k_scales),
+                      _ptr(self.v_scales), _ptr(self.lens), _ptr(counts), 1 if causal else 0, B, n, H, self.kv_heads, D,
+                      self.blocks, self._bound, _kv_strides(q), _kv_strides(out), scale, _ptr(ws), ws_bytes, _stream(dev))
+        return out
 
     # ----------------------------------------------- codes in token order
     def _order(self):
@@ -159,6 +183,7 @@ class Int8KVCache:
             codes[:, :, :nb] = blocks.permute(0, 3, 1, 2, 4).reshape(B, H, nb, BLOCK * D)[..., back]
             scales[:, :, :nb] = s.transpose(1, 2)
         self.lens.copy_(lens)
+        self._bound = nb * BLOCK
 
     def save_codes(self):
         """(k_codes, k_scales, v_codes, v_scales, lens) as ``load_codes`` takes them; copies."""

@@ -135,3 +135,28 @@ def test_cache_block_order_is_a_permutation(D):
     toks[val.reshape(-1)] = torch.arange(64 * D) // D
     assert toks[:16].tolist() == [0, 1, 2, 3, 8, 9, 10, 11, 16, 17, 18, 19, 24, 25, 26, 27]
     assert toks[32 * 16:33 * 16].tolist() == [4, 5, 6, 7, 12, 13, 14, 15, 20, 21, 22, 23, 28, 29, 30, 31]
+
+
+def test_attention_kv_refusals():
+    q, k = torch.zeros(2, 5, 4, 64, dtype=torch.float16), torch.zeros(2, 9, 2, 64, dtype=torch.float16)
+    lens, mask = torch.zeros(2, dtype=torch.int32), torch.ones(2, 9, dtype=torch.bool)
+    for args, kw, msg in (((q, k, k[:, :8]), {}, "k and v must be"), ((q[0], k, k), {}, "q must be"),
+                          ((q.float(), k, k), {}, "data type"), ((q, k.bfloat16(), k), {}, "k and v must be"),
+                          ((q[:, :, :3], k, k), {}, "not a multiple"), ((q[..., :32], k, k), {}, "q must be"),
+                          ((q[:1], k, k), {}, "k must be"), ((q, k, k), dict(scale=0.0), "scale"),
+                          ((q, k, k), dict(scale=float("nan")), "scale"), ((q, k, k), dict(scale=-1.0), "scale"),
+                          ((q, k, k), dict(kv_lens=lens.long()), "kv_lens"), ((q, k, k), dict(kv_lens=lens[:1]), "kv_lens"),
+                          ((q, k, k), dict(key_mask=mask.int()), "key_mask"), ((q, k, k), dict(key_mask=mask[:, :8]), "key_mask"),
+                          ((q, k, k), dict(out=q.float()), "out must be"), ((q, k, k), dict(out=q[:, :4]), "out must be"),
+                          ((q, k, k), dict(out=q[:, :1].expand(2, 5, 4, 64)), "out must be"),
+                          ((q, k, k), dict(out=torch.zeros(2, 5, 4, 66).half()[..., 1:65]), "8-byte"),
+                          ((q, k, k), {}, "GPU only")):
+        with pytest.raises(RuntimeError, match=msg):
+            E.cross_attention(*args, **kw)
+    c = Int8KVCache(2, 2, 64, 100, device="cpu")
+    for args, kw, msg in (((q[:1],), {}, "q must be"), ((torch.zeros(2, 5, 4, 128).half(),), {}, "q must be"),
+                          ((q[:, :, :3],), {}, "not a multiple"), ((q,), dict(counts=lens.long()), "counts"),
+                          ((q,), dict(scale=float("inf")), "scale"), ((q,), dict(out=q[:, :2]), "out must be"),
+                          ((q,), {}, "GPU only")):
+        with pytest.raises(RuntimeError, match=msg):
+            c.attention(*args, **kw)
