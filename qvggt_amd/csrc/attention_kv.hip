@@ -43,7 +43,9 @@ struct KvAttn {
   const int32_t *lens, *counts;
   const uint8_t* mask;
   long mask_bs;
-  int B, Lq, H, Hk, G, Lk, blocks, causal, splits, row_tiles;
+  int B, Lq, H, Hk, G, Lk, blocks, causal;
+  int splits, split_tiles;   // splits of a sequence, key tiles of one: at least split_tiles
+  int row_tiles;
   long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
   float scale_log2;
 };
@@ -219,7 +221,7 @@ template <bool BF, int D, int KB, bool FENCE, class Slot>
 __device__ __forceinline__ void kv_softmax(f32x16 (&sc)[KB], float c, KvState<D>& s, uint4 (&pf)[2 * KB], Slot&& slot) {
   constexpr int W = 8 * KB;
   uint32_t pw[W];
-  float t = 0.f;
+  float t = 0.f, t1 = 0.f;          // two chains
   auto word = [&](int w, float ref) __attribute__((always_inline)) {
     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[w >> 3][2 * (w & 7)], c, -ref));
     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[w >> 3][2 * (w & 7) + 1], c, -ref));
@@ -231,14 +233,15 @@ __device__ __forceinline__ void kv_softmax(f32x16 (&sc)[KB], float c, KvState<D>
     slot(i);
     if (i > 0) {
       t = kv_add_pair<BF>(pw[2 * i - 2], t);
-      t = kv_add_pair<BF>(pw[2 * i - 1], t);
+      t1 = kv_add_pair<BF>(pw[2 * i - 1], t1);
     }
     pw[2 * i] = word(2 * i, s.ref);
     pw[2 * i + 1] = word(2 * i + 1, s.ref);
     if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
   }
   t = kv_add_pair<BF>(pw[W - 2], t);
-  t = kv_add_pair<BF>(pw[W - 1], t);
+  t1 = kv_add_pair<BF>(pw[W - 1], t1);
+  t += t1;
   // some p may have passed 2^15 only if its lane's sum did (p >= 0)
   if (__builtin_amdgcn_ballot_w64(!(t <= KV_SUM_LIMIT) || s.m == -INFINITY)) {
     float mx = sc[0][0];
@@ -314,64 +317,100 @@ __device__ __forceinline__ void kv_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff
                : "memory");
 }
 
-// A 16-bit K or V source, tile by tile: the address of the next tile's first row and
-// the bytes left of the sequence from there (what lies behind them reads as zero).
-// 64-bit: a long cache passes the 32 bits of a buffer offset.
+// A 16-bit K or V source, tile by tile (`keys` rows from tile to tile): the address
+// of the next tile's first row, 64-bit (a long cache passes the 32 bits of a buffer
+// offset), and the bytes of it that may be read: the rest of the sequence, what lies
+// behind reads as zero.
 struct KvSource {
   const uint8_t* at;
-  int64_t left, step;
-  uint32_t row;           // bytes from row to row
-  __device__ __forceinline__ void init(const uint16_t* base, long ts, int D, int len, int64_t key0, int keys) {
+  int64_t step;
+  int left, keys;         // keys left of the sequence
+  uint32_t row, dims;     // bytes from row to row, of a row
+  __device__ __forceinline__ void init(const uint16_t* base, long ts, int D, int len, int64_t key0, int step_keys) {
     at = reinterpret_cast<const uint8_t*>(base) + key0 * ts * 2;
-    left = ((len - 1 - key0) * ts + D) * 2;
-    step = (int64_t)keys * ts * 2;
+    step = (int64_t)step_keys * ts * 2;
+    left = (int)(len - key0);
+    keys = step_keys;
     row = (uint32_t)(ts * 2);
+    dims = 2 * D;
   }
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
-    const int64_t n = left < 0 ? 0 : left > 0xFFFFFFFFll ? 0xFFFFFFFFll : left;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), (short)0, (int)(uint32_t)n, 0x00020000);
+  // descriptor over the first `most` keys (at most 64, of under 2^25 bytes each: 32 bits hold them)
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(int most) const {
+    const int k = left < most ? left : most;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), (short)0, k > 0 ? (int)((k - 1) * row + dims) : 0,
+                                             0x00020000);
   }
-  __device__ __forceinline__ void next() { at += step, left -= step; }
+  __device__ __forceinline__ void next() { at += step, left -= keys; }
 };
 
-// The sequence's keys, queries and the tiles of a row tile's split.
+__device__ __forceinline__ int kv_len(const KvAttn& a, int b) {
+  if (!a.lens) return a.Lk;
+  const int l = a.lens[b];
+  return l < 0 ? 0 : l > a.Lk ? a.Lk : l;
+}
+
+__device__ __forceinline__ int kv_tiles(int len) { return (len + KV_BLOCK - 1) / KV_BLOCK; }
+
+// Which part a workgroup of the wide and pipelined forms takes.  In the order (row tile,
+// split, key head, sequence) fours of neighbours, which mostly read the same keys, share
+// an XCD and its L2, and the fours go round the 8 XCDs.  (Whole sets of row tiles to an
+// XCD do not go evenly into its 64 places: sets of 17 over sequences of 6017 and 2053
+// tokens left some XCDs with 68 workgroups, a second round, and others with 51.)
+constexpr int KV_NEAR = 4;
+struct KvPart {
+  int b, hk, split, rt;
+  bool any;
+};
+__device__ __forceinline__ KvPart kv_part(const KvAttn& a) {
+  const uint32_t x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  uint32_t g = i / KV_NEAR * (8 * KV_NEAR) + x * KV_NEAR + i % KV_NEAR;
+  KvPart p;
+  p.rt = g % a.row_tiles;
+  g /= a.row_tiles;
+  p.split = g % a.splits;
+  g /= a.splits;
+  p.hk = g % a.Hk;
+  p.b = g / a.Hk;
+  p.any = p.b < a.B;
+  return p;
+}
+
+// The sequence's keys and queries, and the tiles of a split, for rows that see at most
+// the keys of query `last_query` (of first_query on): splits lie at the same keys for all
+// row tiles, and grow where the sequence is longer than the host knew.
 struct KvRange {
   int len, nq, t0, t1;
 };
-__device__ __forceinline__ KvRange kv_range(const KvAttn& a, int b, int row0, int rows_tile, int split) {
+__device__ __forceinline__ KvRange kv_range(const KvAttn& a, int b, int split, int first_query, int last_query) {
   KvRange r;
-  r.len = a.Lk;
-  if (a.lens) {
-    const int l = a.lens[b];
-    r.len = l < 0 ? 0 : l > a.Lk ? a.Lk : l;
-  }
+  r.len = kv_len(a, b);
   r.nq = a.Lq;
   if (a.counts) {
     const int c = a.counts[b];
     r.nq = c < 0 ? 0 : c > a.Lq ? a.Lq : c;
   }
-  int last = r.len;                       // keys that the tile's last row sees
+  int last = r.len;                       // keys that the last row sees
   if (a.causal) {
-    int qi = (row0 + rows_tile - 1) / a.G;
-    qi = qi < r.nq ? qi : r.nq - 1;
-    last = r.len - r.nq + qi + 1;
+    last = r.len - r.nq + min(last_query, r.nq - 1) + 1;
     last = last < 0 ? 0 : last > r.len ? r.len : last;
   }
-  const int nt = row0 / a.G < r.nq ? (last + KV_BLOCK - 1) / KV_BLOCK : 0;
-  r.t0 = (int)((long)nt * split / a.splits);
-  r.t1 = (int)((long)nt * (split + 1) / a.splits);
+  const int nt = first_query < r.nq ? kv_tiles(last) : 0;
+  int per = a.split_tiles;
+  if ((long)per * a.splits < kv_tiles(r.len)) per = (kv_tiles(r.len) + a.splits - 1) / a.splits;
+  r.t0 = min((long)nt, (long)split * per);
+  r.t1 = min((long)nt, (long)(split + 1) * per);
   return r;
 }
 
 // Store a lane's row: the quotient to out, or to the split's part with m and l.
 template <bool BF16, int D>
-__device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, float l, int ve, int b, int hk, int row,
-                                         int split, int h, bool live) {
+__device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, float l, int ve, const KvPart& p, int row,
+                                         int h, bool live) {
   if (!live) return;
   const float inv = l == 0.f ? 0.f : __builtin_ldexpf(1.0f / l, ve);
-  const int qi = row / a.G, head = hk * a.G + row % a.G;
+  const int qi = row / a.G, head = p.hk * a.G + row % a.G;
   if (a.splits == 1) {
-    uint16_t* op = a.out + b * a.o_bs + qi * a.o_ts + head * a.o_hs;
+    uint16_t* op = a.out + p.b * a.o_bs + qi * a.o_ts + head * a.o_hs;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -382,9 +421,9 @@ __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, f
         *reinterpret_cast<uint2*>(op + 32 * db + 8 * g + 4 * h) = w;
       }
   } else {
-    const long rows = (long)a.B * a.H * a.Lq;
-    const long at = (long)split * rows + ((long)b * a.Hk + hk) * ((long)a.Lq * a.G) + row;
+    const long at = (((long)p.b * a.splits + p.split) * a.Hk + p.hk) * ((long)a.Lq * a.G) + row;
     float* pp = a.part + at * D;
+    if (l != 0.f)                                    // the join reads no part without a sum
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -395,246 +434,466 @@ __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, f
   }
 }
 
-// ------------------------------------------------------------------ wide form
-template <bool KV8, bool BF16, int D, int QB>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QB == 1 && D == 64 ? 3 : 2, QB == 1 && D == 64 ? 3 : 2))) void kv_attn_wide_kernel(const KvAttn a) {
+// ------------------------------------------------------------------ staging
+// Tiles of K (V = false) or V in LDS, in order, by the whole workgroup.  16-bit: LDS
+// DMA, swizzled rows.  8-bit: codes through registers, decoded once, fragment order.
+template <bool KV8, int D, bool V>
+struct KvTiles {
+  static constexpr int TILE = KV_BLOCK * D * 2;      // bytes
+  static constexpr int DMA = TILE / 1024 / 4;        // 1 KB copies of a wave
+  static constexpr int RPD = 1024 / (2 * D);         // rows of a copy
+  static constexpr int UNITS = KV_BLOCK * D / 16 / 256;   // 16-byte units of a thread
+  KvSource src;
+  uint32_t voff[DMA];
+  const uint4* codes;
+  __device__ __forceinline__ void init(const KvAttn& a, int b, int hk, const KvRange& rg, int wave, int lane) {
+    if constexpr (KV8) {
+      const long block = ((long)b * a.Hk + hk) * a.blocks + rg.t0;
+      codes = reinterpret_cast<const uint4*>(V ? a.vc : a.kc) + block * (KV_BLOCK * D / 16) + wave * 64 + lane;
+    } else {
+      if constexpr (V) src.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ts, D, rg.len, (int64_t)rg.t0 * KV_BLOCK, KV_BLOCK);
+      else src.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ts, D, rg.len, (int64_t)rg.t0 * KV_BLOCK, KV_BLOCK);
+#pragma unroll
+      for (int w = 0; w < DMA; ++w) {
+        const int r = RPD * (DMA * wave + w) + lane / (D / 8), c = lane % (D / 8);
+        voff[w] = (uint32_t)(lane / (D / 8)) * src.row + ((c ^ (V ? kv_fv<D>(r) : kv_fk<D>(r))) * 16);
+      }
+    }
+  }
+  // the next tile on its way to LDS (16-bit) or registers
+  __device__ __forceinline__ void start(uint32_t lds, int wave, uint4 (&raw)[UNITS]) {
+    if constexpr (KV8) {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) raw[u] = codes[256 * u];
+      codes += KV_BLOCK * D / 16;
+    } else {
+      const auto r = src.rsrc(KV_BLOCK);
+#pragma unroll
+      for (int w = 0; w < DMA; ++w) {
+        const int r0 = RPD * (DMA * wave + w);
+        kv_dma16(r, voff[w], (uint32_t)r0 * src.row, lds + r0 * (2 * D));
+      }
+      src.next();
+    }
+  }
+  static __device__ __forceinline__ void place(uint8_t* lds, _Float16 f, int wave, int lane, const uint4 (&raw)[UNITS]) {
+    uint4* t = reinterpret_cast<uint4*>(lds);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      uint4 lo, hi;
+      kv_decode(raw[u], (f16x2){f, f}, lo, hi);
+      const int at = (4 * u + wave) * 128 + lane;
+      t[at] = lo, t[at + 64] = hi;
+    }
+  }
+};
+
+// ------------------------------------------------------------------ pipelined form
+// 4 waves of 32 rows.  Beside tile j's softmax run the QK of tile j + 1 and the PV of tile
+// j - 1, a few of each in every slot, so that no product stands alone.  K is in LDS two
+// tiles ahead, V comes with its own tile, and the workgroup meets once a tile.
+// LEAD: loads are issued one tile earlier still, for D = 64, whose tiles take less time
+// than a load from beyond the L2 (16-bit: a third LDS stage; 8-bit: a second set of registers).
+template <bool KV8, bool BF16, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_pipe_kernel(const KvAttn a) {
   constexpr bool MBF = BF16 && !KV8;
-  constexpr int TILE = KV_BLOCK * D * 2;             // bytes of a 16-bit K or V tile
-  constexpr int KS = D / 16, NV = D / 32;
+  constexpr int TILE = KV_BLOCK * D * 2;
+  constexpr int KS = D / 16, NV = D / 32, NK = 2 * KS, NF = 4 * NV;
+  constexpr int ROWS = 128, AHEAD = D == 64 ? 2 : 1;         // slots from a fragment's read to its use
+  constexpr int LEAD = 0, STAGES = KV8 ? 2 : 2 + LEAD;
+  using TK = KvTiles<KV8, D, false>;
+  using TV = KvTiles<KV8, D, true>;
+  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[STAGES][TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[STAGES][TILE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  const KvPart part = kv_part(a);
+  if (!part.any) return;
+  const int hk = part.hk, b = part.b;
+  const int nrows = a.Lq * a.G;
+  const int row0 = part.rt * ROWS;
+  const int first_query = row0 / a.G;
+  const KvRange rg = kv_range(a, b, part.split, first_query, (min(nrows, row0 + ROWS) - 1) / a.G);
+  if (first_query >= rg.nq) return;
+  const int wrow = row0 + wave * 32, row = wrow + l32;
+  const bool live = wrow < nrows && wrow / a.G < rg.nq;      // wave-uniform
+  const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
+
+  TK kt;
+  TV vt;
+  kt.init(a, b, hk, rg, wave, lane);
+  vt.init(a, b, hk, rg, wave, lane);
+  const uint32_t klds0 = lds_addr(k_lds), vlds0 = lds_addr(v_lds);
+  // 8-bit: what is on its way to registers.  Block scales come by vector loads: a scalar
+  // load in flight would make every wait for an LDS read wait for it, too.
+  struct Flight {
+    uint4 k[TK::UNITS], v[TV::UNITS];
+    float ks, vs;
+  };
+  Flight fa, fx;
+  Flight& fb = LEAD ? fx : fa;                               // of odd steps
+  const float *ks_at = nullptr, *vs_at = nullptr;
+  if constexpr (KV8) {
+    long at = ((long)b * a.Hk + hk) * a.blocks + rg.t0;
+    asm("" : "+v"(at));
+    ks_at = a.ks + at, vs_at = a.vs + at;
+  }
+  KvUnits units;
+  float ks = 0.f;                                            // of this tile
+  uint8_t mask_byte = 1;
+  auto load_mask = [&](int j) __attribute__((always_inline)) {
+    const int key = (rg.t0 + j) * KV_BLOCK + lane;
+    mask_byte = key < rg.len ? a.mask[b * a.mask_bs + key] : 0;
+  };
+  // step j: K of j + 2 + LEAD, V of j + LEAD, the key scale of j + 1 + LEAD, the mask of j + 1
+  auto feed = [&](int j, Flight& f) __attribute__((always_inline)) {
+    if constexpr (!KV8)
+      if (a.mask && j + 1 < n) load_mask(j + 1);
+    if (j + 2 + LEAD < n) kt.start(klds0 + (j + 2 + LEAD) % STAGES * TILE, wave, f.k);
+    if (j + LEAD < n) {
+      vt.start(vlds0 + (j + LEAD) % STAGES * TILE, wave, f.v);
+      if constexpr (KV8) f.vs = *vs_at++;
+    }
+    if constexpr (KV8)
+      if (j + 1 + LEAD < n) f.ks = *++ks_at;
+  };
+  // K of j + 2 and V of j into LDS
+  auto settle = [&](int j, const Flight& f) __attribute__((always_inline)) {
+    if constexpr (KV8) {
+      if (j + 2 < n) TK::place(k_lds[j & 1], (_Float16)1.0f, wave, lane, f.k);
+      TV::place(v_lds[j & 1], (_Float16)units.fit(f.vs), wave, lane, f.v);
+      ks = f.ks;
+    } else if (LEAD && j + 2 + LEAD < n) {
+      static_assert(!LEAD || 2 * TK::DMA == 4, "copies of one step, which may stay in flight");
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    lds_barrier();
+  };
+  // tiles below edge are seen whole by all rows of the wave
+  const int wfirst = wrow / a.G;
+  const int edge = !KV8 && a.mask ? 0 : (a.causal ? min(rg.len, rg.len - rg.nq + wfirst + 1) : rg.len) / KV_BLOCK - rg.t0;
+  auto visible = [&](int j) __attribute__((always_inline)) {
+    uint64_t seen = ~0ull;
+    if (j >= edge) {
+      seen = kv_below(rg.len - (rg.t0 + j) * KV_BLOCK);
+      if constexpr (!KV8)
+        if (a.mask) seen = __builtin_amdgcn_ballot_w64(mask_byte != 0);
+    }
+    return seen;
+  };
+  // value rows of a tile whose keys are left out may hold anything
+  auto clear = [&](int j, uint64_t seen) __attribute__((always_inline)) {
+    if constexpr (!KV8) {
+      if (seen != ~0ull) {
+        uint4* t = reinterpret_cast<uint4*>(v_lds[j % STAGES]);
+#pragma unroll
+        for (int i = 0; i < TILE / 16 / 256; ++i) {
+          constexpr int ROWS_AT = 256 / (D / 8);     // rows that 256 chunks cover
+          const int row = ROWS_AT * i + tid / (D / 8);
+          if (!((uint32_t)(seen >> (ROWS_AT * i / 32 * 32)) >> (row & 31) & 1)) t[256 * i + tid] = make_uint4(0, 0, 0, 0);
+        }
+        lds_barrier();
+      }
+    }
+  };
+  KvState<D> s;
+  s.init();
+  int ve = 0;                                        // of O
+  if (n > 0) {
+    // K of tiles 0 and 1; zero in the stage that the first PV reads (its P is zero, too)
+    kt.start(klds0, wave, fa.k);
+    if constexpr (KV8) {
+      ks = *ks_at;
+      TK::place(k_lds[0], (_Float16)1.0f, wave, lane, fa.k);
+    }
+    if (n > 1) {
+      kt.start(klds0 + TILE, wave, fa.k);
+      if constexpr (KV8) TK::place(k_lds[1], (_Float16)1.0f, wave, lane, fa.k);
+    }
+    if constexpr (LEAD) feed(-1, fb);
+    else if constexpr (!KV8)
+      if (a.mask) load_mask(0);
+    for (int i = tid; i < TILE / 16; i += 256) reinterpret_cast<uint4*>(v_lds[STAGES - 1])[i] = make_uint4(0, 0, 0, 0);
+    if constexpr (!KV8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    uint64_t before = ~0ull;                         // what the tile before left
+    if (!live) {
+      // rows past the end: the wave only stages its share
+      lds_barrier();
+      for (int j = 0; j < n; j += 2) {
+        clear(j - 1, before);
+        before = visible(j);
+        feed(j, fa);
+        settle(j, fb);
+        if (j + 1 < n) {
+          clear(j, before);
+          before = visible(j + 1);
+          feed(j + 1, fb);
+          settle(j + 1, fa);
+        }
+      }
+      clear(n - 1, before);
+      return;
+    }
+    KvRows<KV8, BF16, D> qr;
+    const int rc = row < nrows ? row : nrows - 1;
+    const int qi = rc / a.G;
+    qr.load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc % a.G) * a.q_hs, h, a.scale_log2);
+    const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;                      // the last key that the row sees
+    auto frag_k = [&](int stage, int f) __attribute__((always_inline)) {               // f = kb + 2 st
+      if constexpr (KV8) return reinterpret_cast<const uint4*>(k_lds[stage])[((f & 1) * KS + (f >> 1)) * 64 + lane];
+      else return kv_frag_k<D>(k_lds[stage], f & 1, f >> 1, h, l32);
+    };
+    auto frag_v = [&](int stage, int f) __attribute__((always_inline)) {               // f = db + NV st
+      if constexpr (KV8) return reinterpret_cast<const uint4*>(v_lds[stage])[((f % NV) * 4 + f / NV) * 64 + lane];
+      else return kv_frag_v<D>(v_lds[stage], f % NV, f / NV, lane);
+    };
+    f32x16 sa[2], sb[2];
+    uint4 pa[4] = {}, pb[4];
+#pragma unroll
+    for (int f = 0; f < NK; ++f) sa[f & 1] = kv_mfma<MBF>(frag_k(0, f), qr.f[f >> 1], f < 2 ? f32x16{} : sa[f & 1]);
+    lds_barrier();                                   // the first K stage may be written again
+    auto rescale = [&]() __attribute__((always_inline)) {
+      if constexpr (KV8) {
+        if (units.ve != ve) {
+          s.scale(__builtin_ldexpf(1.0f, ve - units.ve));
+          ve = units.ve;
+        }
+      }
+    };
+    // sc, p: the tile's scores, the probabilities of the tile before; next, pn: the next of each
+    auto step = [&](int j, f32x16 (&sc)[2], f32x16 (&next)[2], uint4 (&p)[4], uint4 (&pn)[4], Flight& out,
+                    const Flight& in) __attribute__((always_inline)) {
+      const int key0 = (rg.t0 + j) * KV_BLOCK;
+      const int ks_stage = (j + 1) % STAGES, vs_stage = (j + STAGES - 1) % STAGES;
+      constexpr int PK = NK / 8, PV = NF / 8;        // products of a slot
+      uint4 kf[NK], vf[NF];
+      clear(j + STAGES - 1, before);
+      auto read = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < PK; ++e) kf[slot * PK + e] = frag_k(ks_stage, slot * PK + e);
+#pragma unroll
+        for (int e = 0; e < PV; ++e) vf[slot * PV + e] = frag_v(vs_stage, slot * PV + e);
+      };
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) read(i);
+      const uint64_t seen = visible(j);
+      const float kscale = ks;
+      feed(j, out);
+      rescale();
+      const float c = KV8 ? kv_factor((kscale > 0.f || kscale != kscale ? kscale : 1.0f) * qr.mul) : qr.mul;
+      if (j >= edge) kv_mask<2>(sc, seen & kv_below(upto - key0 + 1), h);
+      kv_softmax<MBF, D, 2, true>(sc, c, s, pn, [&](int i) __attribute__((always_inline)) {
+        if (i + AHEAD < 8) read(i + AHEAD);
+#pragma unroll
+        for (int e = 0; e < PK; ++e) {
+          const int f = i * PK + e;
+          next[f & 1] = kv_mfma<MBF>(kf[f], qr.f[f >> 1], f < 2 ? f32x16{} : next[f & 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+          const int f = i * PV + e;
+          s.o[f % NV] = kv_mfma<MBF>(vf[f], p[f / NV], s.o[f % NV]);
+        }
+      });
+      before = seen;
+      settle(j, in);
+    };
+    auto last = [&](uint4 (&p)[4]) __attribute__((always_inline)) {
+      clear(n - 1, before);
+      rescale();
+#pragma unroll
+      for (int f = 0; f < NF; ++f) s.o[f % NV] = kv_mfma<MBF>(frag_v((n - 1) % STAGES, f), p[f / NV], s.o[f % NV]);
+    };
+    int j = 0;
+    for (; j + 1 < n; j += 2) {
+      step(j, sa, sb, pa, pb, fa, fb);
+      step(j + 1, sb, sa, pb, pa, fb, fa);
+    }
+    if (j < n) {
+      step(j, sa, sb, pa, pb, fa, fb);
+      last(pb);
+    } else {
+      last(pa);
+    }
+  } else if (!live) {
+    return;
+  }
+  kv_store<BF16, D>(a, s, kv_half_sum(s.l), ve, part, row, h, row < nrows && row / a.G < rg.nq);
+}
+
+// ------------------------------------------------------------------ wide form
+// 4 waves of 64 rows (two blocks of 32), D = 64: every fragment that is read from LDS and
+// every code that is decoded serves twice the rows.  Inside a tile the second block's QK
+// runs beside the first one's softmax, the first one's PV beside the second's.
+template <bool KV8, bool BF16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_wide_kernel(const KvAttn a) {
+  constexpr int D = 64, QB = 2;
+  constexpr bool MBF = BF16 && !KV8;
+  constexpr int TILE = KV_BLOCK * D * 2;
   constexpr int ROWS = 4 * 32 * QB;
+  using TK = KvTiles<KV8, D, false>;
+  using TV = KvTiles<KV8, D, true>;
   __shared__ __attribute__((aligned(1024))) uint8_t k_lds[2][TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v_lds[2][TILE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
-  // consecutive row tiles of one (sequence, key head, split) share an XCD and its L2
-  const int lid = xcd_remap(blockIdx.x, gridDim.x);
-  const int rt = lid % a.row_tiles;
-  const int split = lid / a.row_tiles % a.splits;
-  const int hk = lid / (a.row_tiles * a.splits) % a.Hk;
-  const int b = lid / (a.row_tiles * a.splits * a.Hk);
+  const KvPart part = kv_part(a);
+  if (!part.any) return;
+  const int hk = part.hk, b = part.b;
   const int nrows = a.Lq * a.G;
-  const int row0 = rt * ROWS;
-  const KvRange rg = kv_range(a, b, row0, nrows - row0 < ROWS ? nrows - row0 : ROWS, split);
-  if (row0 / a.G >= rg.nq) return;
+  const int row0 = part.rt * ROWS;
+  const int first_query = row0 / a.G;
+  const KvRange rg = kv_range(a, b, part.split, first_query, (min(nrows, row0 + ROWS) - 1) / a.G);
+  if (first_query >= rg.nq) return;
   const int wrow = row0 + wave * 32 * QB;
   const bool live = wrow < nrows && wrow / a.G < rg.nq;      // wave-uniform
+  const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
 
-  KvRows<KV8, BF16, D> qr[QB];
-  KvState<D> s[QB];
-  int row[QB], upto[QB];                             // upto: the last key that the row sees
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    row[qb] = wrow + 32 * qb + l32;
-    const int rc = row[qb] < nrows ? row[qb] : nrows - 1;
-    const int qi = rc / a.G, head = hk * a.G + rc % a.G;
-    qr[qb].load(a.q + b * a.q_bs + qi * a.q_ts + head * a.q_hs, h, a.scale_log2);
-    upto[qb] = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
-    s[qb].init();
-  }
-  const int first_upto = a.causal ? rg.len - rg.nq + wrow / a.G : rg.len - 1;    // of the wave's first row
-
-  // ---- tiles of the 16-bit source
-  constexpr int DMA = TILE / 1024 / 4;               // 1 KB copies of a wave for K and for V
-  constexpr int RPD = 1024 / (2 * D);                // rows of a copy
+  TK kt;
+  TV vt;
+  kt.init(a, b, hk, rg, wave, lane);
+  vt.init(a, b, hk, rg, wave, lane);
   const uint32_t klds0 = lds_addr(k_lds), vlds0 = lds_addr(v_lds);
-  KvSource sk, sv;
-  uint32_t k_voff[DMA], v_voff[DMA];
-  if constexpr (!KV8) {
-    const int64_t key0 = (int64_t)rg.t0 * KV_BLOCK;
-    sk.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ts, D, rg.len, key0, KV_BLOCK);
-    sv.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ts, D, rg.len, key0, KV_BLOCK);
-#pragma unroll
-    for (int w = 0; w < DMA; ++w) {
-      const int r = RPD * (DMA * wave + w) + lane / (D / 8), c = lane % (D / 8);
-      k_voff[w] = (uint32_t)(lane / (D / 8)) * sk.row + ((c ^ kv_fk<D>(r)) * 16);
-      v_voff[w] = (uint32_t)(lane / (D / 8)) * sv.row + ((c ^ kv_fv<D>(r)) * 16);
-    }
+  uint4 kraw[TK::UNITS], vraw[TV::UNITS];
+  const float *ks_at = nullptr, *vs_at = nullptr;            // by vector loads: see the pipelined form
+  if constexpr (KV8) {
+    long at = ((long)b * a.Hk + hk) * a.blocks + rg.t0;
+    asm("" : "+v"(at));
+    ks_at = a.ks + at, vs_at = a.vs + at;
   }
-  auto issue16 = [&](int buf) __attribute__((always_inline)) {      // the next tile
-    const auto rk = sk.rsrc(), rv = sv.rsrc();
-#pragma unroll
-    for (int w = 0; w < DMA; ++w) {
-      const int r0 = RPD * (DMA * wave + w);
-      kv_dma16(rk, k_voff[w], (uint32_t)r0 * sk.row, klds0 + buf * TILE + r0 * (2 * D));
-      kv_dma16(rv, v_voff[w], (uint32_t)r0 * sv.row, vlds0 + buf * TILE + r0 * (2 * D));
-    }
-    sk.next();
-    sv.next();
-  };
-  // ---- tiles of the cache: 16 codes a thread and step, one 16-byte unit
-  constexpr int UNITS = KV_BLOCK * D / 16 / 256;     // of a thread for K and for V
-  const long cache0 = ((long)b * a.Hk + hk) * a.blocks;
-  uint4 kraw[UNITS], vraw[UNITS];
-  float ks_next = 0.f, vs_next = 0.f;
-  auto fetch8 = [&](int tile) __attribute__((always_inline)) {
-    const uint4* kp = reinterpret_cast<const uint4*>(a.kc) + (cache0 + tile) * (KV_BLOCK * D / 16);
-    const uint4* vp = reinterpret_cast<const uint4*>(a.vc) + (cache0 + tile) * (KV_BLOCK * D / 16);
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      kraw[u] = kp[256 * u + tid];
-      vraw[u] = vp[256 * u + tid];
-    }
-    ks_next = a.ks[cache0 + tile];
-    vs_next = a.vs[cache0 + tile];
-  };
   KvUnits units;
-  auto place8 = [&](int buf) __attribute__((always_inline)) {
-    const _Float16 f = (_Float16)units.fit(vs_next);
-    uint4* kt = reinterpret_cast<uint4*>(k_lds[buf]);
-    uint4* vt = reinterpret_cast<uint4*>(v_lds[buf]);
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int unit = 256 * u + tid, at = (unit >> 6) * 128 + (unit & 63);
-      uint4 lo, hi;
-      kv_decode(kraw[u], (f16x2){(_Float16)1.0f, (_Float16)1.0f}, lo, hi);
-      kt[at] = lo, kt[at + 64] = hi;
-      kv_decode(vraw[u], (f16x2){f, f}, lo, hi);
-      vt[at] = lo, vt[at + 64] = hi;
-    }
-  };
-  auto frag_k = [&](int buf, int kb, int st) __attribute__((always_inline)) {
-    if constexpr (KV8) return reinterpret_cast<const uint4*>(k_lds[buf])[(kb * KS + st) * 64 + lane];
-    else return kv_frag_k<D>(k_lds[buf], kb, st, h, l32);
-  };
-  auto frag_v = [&](int buf, int db, int st) __attribute__((always_inline)) {
-    if constexpr (KV8) return reinterpret_cast<const uint4*>(v_lds[buf])[(db * 4 + st) * 64 + lane];
-    else return kv_frag_v<D>(v_lds[buf], db, st, lane);
-  };
-
-  // One tile.  At most 8 K and then 8 V fragments are held at a time (32 registers each).
-  // QB = 2: the first block's QK, then the second's beside the first's softmax, the
-  // first's PV beside the second's softmax.
-  auto compute = [&](int buf, const float (&c)[QB], bool masked, uint64_t seen, int key0) __attribute__((always_inline)) {
-    f32x16 sc[QB][2];
-    uint4 pf[QB][4];
-    constexpr int KG = KS / 4, VG = NV * 4 / 8;      // groups of 8 fragments
-    uint4 kf[KG][8], vf[VG][8];
-    auto read_k = [&](int g) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) kf[g][i] = frag_k(buf, i & 1, 4 * g + (i >> 1));
-    };
-    auto read_v = [&](int g, int i) __attribute__((always_inline)) {
-      const int f = 8 * g + i;
-      vf[g][i] = frag_v(buf, f % NV, f / NV);
-    };
-    auto qk = [&](int qb, int f) __attribute__((always_inline)) {    // f = 0 .. 2 KS - 1
-      const int kb = f & 1, st = f >> 1;
-      sc[qb][kb] = kv_mfma<MBF>(kf[f / 8][f % 8], qr[qb].f[st], st == 0 ? f32x16{} : sc[qb][kb]);
-    };
-    auto pv = [&](int qb, int f) __attribute__((always_inline)) {    // f = 0 .. 4 NV - 1
-      s[qb].o[f % NV] = kv_mfma<MBF>(vf[f / 8][f % 8], pf[qb][f / NV], s[qb].o[f % NV]);
-    };
-    auto mask = [&](int qb) __attribute__((always_inline)) {
-      if (masked) kv_mask<2>(sc[qb], seen & kv_below(upto[qb] - key0 + 1), h);
-    };
-    read_k(0);
-#pragma unroll
-    for (int g = 0; g < KG; ++g) {
-      if (g + 1 < KG) read_k(g + 1);
-      if constexpr (KG > 1) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) qk(0, 8 * g + i);
-    }
-    mask(0);
-    if constexpr (QB == 2) {
-      static_assert(QB == 1 || (KG == 1 && VG == 1), "two row blocks: D = 64");
-      kv_softmax<MBF, D, 2, true>(sc[0], c[0], s[0], pf[0], [&](int i) __attribute__((always_inline)) {
-        qk(1, i);
-        if (i >= 4) {
-          read_v(0, 2 * (i - 4));
-          read_v(0, 2 * (i - 4) + 1);
-        }
-      });
-      mask(1);
-      kv_softmax<MBF, D, 2, true>(sc[1], c[1], s[1], pf[1], [&](int i) __attribute__((always_inline)) { pv(0, i); });
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pv(1, i);
-    } else {
-      kv_softmax<MBF, D, 2, (VG > 1)>(sc[0], c[0], s[0], pf[0], [&](int i) __attribute__((always_inline)) {
-        if (i >= 4) {
-          read_v(0, 2 * (i - 4));
-          read_v(0, 2 * (i - 4) + 1);
-        }
-      });
-#pragma unroll
-      for (int g = 0; g < VG; ++g) {
-        if (g + 1 < VG)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) read_v(g + 1, i);
-        if constexpr (VG > 1) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pv(0, 8 * g + i);
-      }
-    }
-  };
-
-  int ve = 0;                                        // of O
-  float ks = 0.f;
+  float ks = 0.f, ks_next = 0.f, vs_next = 0.f;
   uint8_t mask_byte = 1;
-  auto load_mask = [&](int tile) __attribute__((always_inline)) {
-    const int key = tile * KV_BLOCK + lane;
-    mask_byte = key < rg.len ? a.mask[b * a.mask_bs + key] : 0;
-  };
-  if (rg.t0 < rg.t1) {
+  // the tile on its way (into stage j % 2), and into place
+  auto feed = [&](int j) __attribute__((always_inline)) {
+    kt.start(klds0 + (j & 1) * TILE, wave, kraw);
+    vt.start(vlds0 + (j & 1) * TILE, wave, vraw);
     if constexpr (KV8) {
-      fetch8(rg.t0);
-      place8(0);
+      ks_next = *ks_at++, vs_next = *vs_at++;
+    } else if (a.mask) {
+      const int key = (rg.t0 + j) * KV_BLOCK + lane;
+      mask_byte = key < rg.len ? a.mask[b * a.mask_bs + key] : 0;
+    }
+  };
+  auto settle = [&](int j) __attribute__((always_inline)) {
+    if constexpr (KV8) {
+      TK::place(k_lds[j & 1], (_Float16)1.0f, wave, lane, kraw);
+      TV::place(v_lds[j & 1], (_Float16)units.fit(vs_next), wave, lane, vraw);
       ks = ks_next;
     } else {
-      issue16(0);
-      if (a.mask) load_mask(rg.t0);
-      __builtin_amdgcn_s_waitcnt(0x0F70);            // vmcnt(0)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    lds_barrier();
-  }
-  for (int tile = rg.t0; tile < rg.t1; ++tile) {
-    const int buf = (tile - rg.t0) & 1, key0 = tile * KV_BLOCK;
-    const bool more = tile + 1 < rg.t1;
-    uint64_t seen = kv_below(rg.len - key0);
+  };
+  // tiles below edge are seen whole by all rows of the wave
+  const int edge =
+      !KV8 && a.mask ? 0 : (a.causal ? min(rg.len, rg.len - rg.nq + wrow / a.G + 1) : rg.len) / KV_BLOCK - rg.t0;
+  // the keys of tile j that are there; value rows of the others may hold anything
+  auto visible = [&](int j) __attribute__((always_inline)) {
+    uint64_t seen = kv_below(rg.len - (rg.t0 + j) * KV_BLOCK);
     if constexpr (!KV8) {
-      if (a.mask) {
-        seen = __builtin_amdgcn_ballot_w64(mask_byte != 0);
-        if (more) load_mask(tile + 1);
-      }
-      if (seen != ~0ull) {                           // value rows that are left out may hold anything
-        for (int i = tid; i < TILE / 16; i += 256)
-          if (!((seen >> (i / (D / 8))) & 1)) reinterpret_cast<uint4*>(v_lds[buf])[i] = make_uint4(0, 0, 0, 0);
+      if (a.mask) seen = __builtin_amdgcn_ballot_w64(mask_byte != 0);
+      if (seen != ~0ull) {
+        uint4* t = reinterpret_cast<uint4*>(v_lds[j & 1]);
+#pragma unroll
+        for (int i = 0; i < TILE / 16 / 256; ++i) {
+          constexpr int ROWS_AT = 256 / (D / 8);     // rows that 256 chunks cover
+          const int row = ROWS_AT * i + tid / (D / 8);
+          if (!((uint32_t)(seen >> (ROWS_AT * i / 32 * 32)) >> (row & 31) & 1)) t[256 * i + tid] = make_uint4(0, 0, 0, 0);
+        }
         lds_barrier();
       }
     }
-    if (more) {
-      if constexpr (KV8) fetch8(tile + 1);
-      else issue16(buf ^ 1);
+    return seen;
+  };
+  if (n > 0) {
+    feed(0);
+    settle(0);
+  }
+  if (!live) {
+    // rows past the end: the wave only stages its share
+    for (int j = 0; j < n; ++j) {
+      lds_barrier();
+      visible(j);
+      if (j + 1 < n) {
+        feed(j + 1);
+        settle(j + 1);
+      }
     }
-    if (live && seen) {
-      float c[QB];
+    return;
+  }
+  KvRows<KV8, BF16, D> qr[QB];
+  KvState<D> s[QB];
+  int upto[QB];                                      // the last key that the row sees
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) c[qb] = KV8 ? kv_factor((ks > 0.f || ks != ks ? ks : 1.0f) * qr[qb].mul) : qr[qb].mul;
-      if constexpr (KV8) {
-        if (units.ve != ve) {
-          const float by = __builtin_ldexpf(1.0f, ve - units.ve);
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = wrow + 32 * qb + l32, rc = r < nrows ? r : nrows - 1;
+    const int qi = rc / a.G;
+    qr[qb].load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc % a.G) * a.q_hs, h, a.scale_log2);
+    upto[qb] = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
+    s[qb].init();
+  }
+  int ve = 0;                                        // of O
+  for (int j = 0; j < n; ++j) {
+    lds_barrier();                                   // tile j is in place, stage j + 1 free
+    const int buf = j & 1;
+    const uint64_t seen = visible(j);
+    float c[QB];
 #pragma unroll
-          for (int qb = 0; qb < QB; ++qb) s[qb].scale(by);
+    for (int qb = 0; qb < QB; ++qb) c[qb] = KV8 ? kv_factor((ks > 0.f || ks != ks ? ks : 1.0f) * qr[qb].mul) : qr[qb].mul;
+    if constexpr (KV8) {
+      if (units.ve != ve) {
+        const float by = __builtin_ldexpf(1.0f, ve - units.ve);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) s[qb].scale(by);
+        ve = units.ve;
+      }
+    }
+    f32x16 sc[QB][2];
+    uint4 pf[QB][4], kf[8], vf[8];
+    auto qk = [&](int qb, int f) __attribute__((always_inline)) {    // f = kb + 2 st
+      sc[qb][f & 1] = kv_mfma<MBF>(kf[f], qr[qb].f[f >> 1], f < 2 ? f32x16{} : sc[qb][f & 1]);
+    };
+    auto pv = [&](int qb, int f) __attribute__((always_inline)) {    // f = db + 2 st
+      s[qb].o[f & 1] = kv_mfma<MBF>(vf[f], pf[qb][f >> 1], s[qb].o[f & 1]);
+    };
+    auto mask = [&](int qb) __attribute__((always_inline)) {
+      if (j >= edge) kv_mask<2>(sc[qb], seen & kv_below(upto[qb] - (rg.t0 + j) * KV_BLOCK + 1), h);
+    };
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+      if constexpr (KV8) kf[f] = reinterpret_cast<const uint4*>(k_lds[buf])[((f & 1) * 4 + (f >> 1)) * 64 + lane];
+      else kf[f] = kv_frag_k<D>(k_lds[buf], f & 1, f >> 1, h, l32);
+    }
+    if (j + 1 < n) feed(j + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < 8; ++f) qk(0, f);
+    mask(0);
+    kv_softmax<MBF, D, 2, true>(sc[0], c[0], s[0], pf[0], [&](int i) __attribute__((always_inline)) {
+      qk(1, i);
+      if (i >= 4)
+#pragma unroll
+        for (int f = 2 * (i - 4); f < 2 * (i - 4) + 2; ++f) {
+          if constexpr (KV8) vf[f] = reinterpret_cast<const uint4*>(v_lds[buf])[((f & 1) * 4 + (f >> 1)) * 64 + lane];
+          else vf[f] = kv_frag_v<D>(v_lds[buf], f & 1, f >> 1, lane);
         }
-      }
-      compute(buf, c, seen != ~0ull || first_upto < key0 + KV_BLOCK - 1, seen, key0);
-    }
-    ve = units.ve;
-    if (more) {
-      if constexpr (KV8) {
-        place8(buf ^ 1);
-        ks = ks_next;
-      } else {
-        __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the next tiles have landed
-      }
-    }
-    lds_barrier();
+    });
+    mask(1);
+    kv_softmax<MBF, D, 2, true>(sc[1], c[1], s[1], pf[1], [&](int i) __attribute__((always_inline)) { pv(0, i); });
+    if (j + 1 < n) settle(j + 1);
+#pragma unroll
+    for (int f = 0; f < 8; ++f) pv(1, f);
   }
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb)
-    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), ve, b, hk, row[qb], split, h,
-                      row[qb] < nrows && row[qb] / a.G < rg.nq);
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = wrow + 32 * qb + l32;
+    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), ve, part, r, h, r < nrows && r / a.G < rg.nq);
+  }
 }
 
 // ------------------------------------------------------------------ step form
@@ -656,11 +915,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
-  const int split = blockIdx.x % a.splits;
-  const int hk = blockIdx.x / a.splits % a.Hk;
-  const int b = blockIdx.x / (a.splits * a.Hk);
+  const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int nrows = a.Lq * a.G;                      // <= 32
-  const KvRange rg = kv_range(a, b, 0, nrows, split);
+  const KvRange rg = kv_range(a, b, split, 0, a.Lq - 1);
   if (rg.nq == 0) return;
   const int rc = l32 < nrows ? l32 : nrows - 1;
   const int qi = rc / a.G;
@@ -735,7 +992,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
     sk.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ts, D, rg.len, (int64_t)tile * KT, KT * C::WAVES);
     sv.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ts, D, rg.len, (int64_t)tile * KT, KT * C::WAVES);
     auto issue = [&](int buf) __attribute__((always_inline)) {      // the wave's next tile
-      const auto rk = sk.rsrc(), rv = sv.rsrc();
+      const auto rk = sk.rsrc(KT), rv = sv.rsrc(KT);
 #pragma unroll
       for (int w = 0; w < DMA; ++w) {
         const int r0 = RPD * w, row = r0 + lane / (D / 8), c = lane % (D / 8);
@@ -832,45 +1089,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
       uint16_t* op = a.out + b * a.o_bs + (row / a.G) * a.o_ts + (hk * a.G + row % a.G) * a.o_hs + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF16>(o.x, o.y), pack2<BF16>(o.z, o.w));
     } else {
-      const long rows = (long)a.B * a.H * a.Lq;
-      *reinterpret_cast<float4*>(a.part + ((long)split * rows + ((long)b * a.Hk + hk) * nrows + row) * D + d) = o;
+      *reinterpret_cast<float4*>(a.part + ((((long)b * a.splits + split) * a.Hk + hk) * nrows + row) * D + d) = o;
     }
   }
   if (a.splits > 1 && wave == 0 && h == 0 && l32 < rows_out) {
-    const long rows = (long)a.B * a.H * a.Lq;
-    a.stat[(long)split * rows + ((long)b * a.Hk + hk) * nrows + l32] = make_float2(m, sum);
+    a.stat[(((long)b * a.splits + split) * a.Hk + hk) * nrows + l32] = make_float2(m, sum);
   }
 }
 
 // ------------------------------------------------------------------ join of the splits
-// A thread takes 4 dims of one row: sum of the splits' quotients, weighted by l 2^m.
+// A thread takes 4 dims of one row: sum of the splits' quotients, weighted by l 2^m, with
+// a running maximum, so that all loads are on their way at once.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttn a) {
-  const long rows = (long)a.B * a.H * a.Lq;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long at = i / (D / 4);
-  if (at >= rows) return;
+  const int b = blockIdx.z, hk = blockIdx.y;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t row = i / (D / 4), per = (uint32_t)a.Lq * a.G;
+  if (row >= per) return;
   const int d = 4 * (int)(i % (D / 4));
-  const int per = a.Lq * a.G;
-  const int row = (int)(at % per), hk = (int)(at / per % a.Hk), b = (int)(at / per / a.Hk);
   const int qi = row / a.G;
   if (a.counts && qi >= a.counts[b]) return;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stat[s * rows + at].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
+  const long rows = (long)a.Hk * per;                // of a split
+  const long at = (long)b * a.splits * rows + (long)hk * per + row;
+  const float2* stat = a.stat + at;
+  const float* part = a.part + at * D + d;
+  float m = -INFINITY, sum = 0.f;
   float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float2 st = a.stat[s * rows + at];
-    const float w = st.y * __builtin_amdgcn_exp2f(st.x - ref);
-    if (w != 0.f) {                                  // NaN counts
-      const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d);
-      sum += w;
-      o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
-    }
+    const float2 st = stat[s * rows];
+    const float4 x = *reinterpret_cast<const float4*>(part + s * rows * D);
+    const float up = fmaxf(m, st.x), ref = up == -INFINITY ? 0.f : up;
+    const float keep = __builtin_amdgcn_exp2f(m - ref), w = st.y * __builtin_amdgcn_exp2f(st.x - ref);
+    m = up;
+    sum = sum * keep + w;
+    // a split that saw nothing (w = 0) has no part; NaN counts
+    o.x = o.x * keep + (w != 0.f ? w * x.x : 0.f), o.y = o.y * keep + (w != 0.f ? w * x.y : 0.f);
+    o.z = o.z * keep + (w != 0.f ? w * x.z : 0.f), o.w = o.w * keep + (w != 0.f ? w * x.w : 0.f);
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  uint16_t* op = a.out + b * a.o_bs + qi * a.o_ts + (hk * a.G + row % a.G) * a.o_hs + d;
+  uint16_t* op = a.out + b * a.o_bs + qi * a.o_ts + (hk * a.G + (int)row % a.G) * a.o_hs + d;
   *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
 }
 
@@ -884,38 +1142,55 @@ struct KvPlan {
 static KvPlan kv_plan(bool kv8, int64_t B, int64_t Lq, int64_t H, int64_t Hk, int64_t D, int64_t keys) {
   const int64_t rows = Lq * (H / Hk), heads = B * Hk, tiles = (keys + KV_BLOCK - 1) / KV_BLOCK;
   KvPlan p = {};
-  int64_t wg, slots, least;
   if (rows <= 32) {
     p.step = true, p.qb = 1, p.row_tiles = 1;
-    wg = heads, slots = kv8 ? 512 : 256, least = 8;         // tiles of a split at least: two a wave
-  } else {
-    p.qb = D == 64 && rows > 128 ? 2 : 1;
-    p.row_tiles = (int)((rows + 128 * p.qb - 1) / (128 * p.qb));
-    wg = heads * p.row_tiles, slots = 512, least = 8;
+    const int64_t slots = kv8 ? 512 : 256;
+    int64_t s = heads < slots ? slots / (heads > 0 ? heads : 1) : 1;
+    if (s > tiles / 8) s = tiles / 8;                       // two tiles a wave at least
+    if (s > 64) s = 64;
+    p.splits = (int)(s < 1 ? 1 : s);
+    return p;
   }
-  int64_t s = wg < slots ? slots / (wg > 0 ? wg : 1) : 1;
-  if (s > tiles / least) s = tiles / least;
-  if (s > 64) s = 64;
-  p.splits = (int)(s < 1 ? 1 : s);
+  p.qb = D == 64 && rows > 128 ? 2 : 1;
+  p.row_tiles = (int)((rows + 128 * p.qb - 1) / (128 * p.qb));
+  const int64_t wg = heads * p.row_tiles;
+  // time of s splits in ns: rounds of 512 workgroups, two a CU (the last cheaper with at
+  // most one a CU), each of its tiles and some 3 tiles' worth of prologue and end; the
+  // join.  Several sequences may be of any lengths: the mean of all full, and of half the
+  // keys spread over the CUs with one sequence still full.
+  const double pair = p.qb == 2 ? 2430 : D == 64 ? 1300 : 2100, one = p.qb == 2 ? 1480 : D == 64 ? 860 : 1240;
+  double best = 1e300;
+  p.splits = 1;
+  for (int64_t s = 1; s <= 64 && s <= (tiles > 1 ? tiles : 1); ++s) {
+    const int64_t n = wg * s, rem = n % 512;
+    const double per = (double)((tiles + s - 1) / s) + 3;
+    double t = (double)(n / 512) * per * pair + (rem == 0 ? 0 : rem <= 256 ? per * one : per * pair);
+    if (B > 1) {
+      const double half = 0.5 * n * per / 512 * pair;
+      t = 0.5 * (t + (half > per * one ? half : per * one));
+    }
+    if (s > 1) t += 4000 + (double)s * B * H * Lq * D * 8 / 8000;
+    if (t < best) best = t, p.splits = (int)s;
+  }
   return p;
 }
 
-static size_t kv_split_bytes(int64_t B, int64_t Lq, int64_t H, int64_t D) { return (size_t)(B * Lq * H) * (D * 4 + 8); }
+static int64_t kv_split_bytes(int64_t B, int64_t Lq, int64_t H, int64_t D) { return B * Lq * H * (D * 4 + 8); }
 
 template <bool KV8, bool BF16, int D>
 static void kv_launch(const KvAttn& a, const KvPlan& p, hipStream_t st) {
-  const unsigned wg = (unsigned)(a.B * a.Hk * p.row_tiles * p.splits);
+  const int64_t n = (int64_t)a.B * a.Hk * p.splits * p.row_tiles, round = 8 * KV_NEAR;
+  const unsigned wg = (unsigned)((n + round - 1) / round * round);
   if (p.step) {
-    hipLaunchKernelGGL((kv_attn_step_kernel<KV8, BF16, D>), dim3(wg), dim3(256), 0, st, a);
-  } else if constexpr (D == 64) {
-    if (p.qb == 2) hipLaunchKernelGGL((kv_attn_wide_kernel<KV8, BF16, D, 2>), dim3(wg), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv_attn_wide_kernel<KV8, BF16, D, 1>), dim3(wg), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv_attn_step_kernel<KV8, BF16, D>), dim3(p.splits, a.Hk, a.B), dim3(256), 0, st, a);
+  } else if (D == 64 && p.qb == 2) {
+    hipLaunchKernelGGL((kv_attn_wide_kernel<KV8, BF16>), dim3(wg), dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((kv_attn_wide_kernel<KV8, BF16, D, 1>), dim3(wg), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv_attn_pipe_kernel<KV8, BF16, D>), dim3(wg), dim3(256), 0, st, a);
   }
   if (p.splits > 1) {
-    const long threads = (long)a.B * a.H * a.Lq * (D / 4);
-    hipLaunchKernelGGL((kv_attn_join_kernel<BF16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+    const long threads = (long)a.G * a.Lq * (D / 4);
+    hipLaunchKernelGGL((kv_attn_join_kernel<BF16, D>), dim3((unsigned)((threads + 255) / 256), a.Hk, a.B), dim3(256), 0, st, a);
   }
 }
 
@@ -944,13 +1219,13 @@ static int kv_common(KvAttn& a, const char* what, const void* q, void* out, int 
 }
 
 // Splits that the workspace holds, and where their parts lie.
-static int kv_place(KvAttn& a, KvPlan& p, int64_t D, void* ws, int64_t ws_bytes) {
-  const size_t per = kv_split_bytes(a.B, a.Lq, a.H, D);
-  if (p.splits > 1 && (!ws || (uintptr_t)ws % 16 || (size_t)ws_bytes / per < 2)) p.splits = 1;
-  if (p.splits > 1 && (size_t)ws_bytes / per < (size_t)p.splits) p.splits = (int)((size_t)ws_bytes / per);
+static int kv_place(KvAttn& a, KvPlan& p, int64_t D, int64_t tiles, void* ws, int64_t ws_bytes) {
+  const int64_t per = kv_split_bytes(a.B, a.Lq, a.H, D);
+  if (p.splits > 1 && (!ws || (uintptr_t)ws % 16)) p.splits = 1;
+  if (p.splits > 1 && p.splits * per > ws_bytes) p.splits = (int)(ws_bytes / per > 1 ? ws_bytes / per : 1);
   a.splits = p.splits, a.row_tiles = p.row_tiles;
-  QV_CHECK_ARG((int64_t)a.B * a.Hk * p.row_tiles * p.splits <= INT32_MAX &&
-                   (int64_t)a.B * a.H * a.Lq * (D / 4) / 256 < INT32_MAX,
+  a.split_tiles = (int)((tiles + p.splits - 1) / p.splits);
+  QV_CHECK_ARG((int64_t)a.B * a.Hk * p.splits * p.row_tiles <= INT32_MAX - 64 && a.B <= 65535 && a.Hk <= 65535,
                "grid too large");
   a.part = (float*)ws;
   a.stat = (float2*)((char*)ws + (size_t)p.splits * a.B * a.Lq * a.H * D * 4);
@@ -963,7 +1238,7 @@ extern "C" int64_t qv_attention_kv_workspace(int cached, int64_t B, int64_t Lq, 
                                              int64_t keys) {
   if (B <= 0 || Lq <= 0 || H <= 0 || Hk <= 0 || H % Hk || keys < 0 || (D != 64 && D != 128)) return 0;
   const qv::KvPlan p = qv::kv_plan(cached != 0, B, Lq, H, Hk, D, keys);
-  return p.splits > 1 ? (int64_t)(p.splits * qv::kv_split_bytes(B, Lq, H, D)) : 0;
+  return p.splits > 1 ? p.splits * qv::kv_split_bytes(B, Lq, H, D) : 0;
 }
 
 #define QV_KV_LAUNCH(KV8)                                                                          \
@@ -997,7 +1272,7 @@ extern "C" int qv_attention_cross(const void* q, const void* k, const void* v, v
     a.lens = lens, a.mask = mask, a.mask_bs = mask_stride;
   }
   qv::KvPlan p = qv::kv_plan(false, B, Lq, H, Hk, D, Lk);
-  if (int rc = qv::kv_place(a, p, D, workspace, workspace_bytes)) return rc;
+  if (int rc = qv::kv_place(a, p, D, (Lk + qv::KV_BLOCK - 1) / qv::KV_BLOCK, workspace, workspace_bytes)) return rc;
   QV_KV_LAUNCH(false)
   return qv::check_launch("attention_cross");
 }
@@ -1019,7 +1294,7 @@ extern "C" int qv_kv8_attention(const void* q, void* out, int dtype, const void*
   a.lens = lens, a.counts = counts, a.causal = causal != 0, a.blocks = (int)blocks;
   if (keys < 0 || keys > blocks * qv::KV_BLOCK) keys = blocks * qv::KV_BLOCK;
   qv::KvPlan p = qv::kv_plan(true, B, Lq, H, Hk, D, keys);
-  if (int rc = qv::kv_place(a, p, D, workspace, workspace_bytes)) return rc;
+  if (int rc = qv::kv_place(a, p, D, (keys + qv::KV_BLOCK - 1) / qv::KV_BLOCK, workspace, workspace_bytes)) return rc;
   QV_KV_LAUNCH(true)
   return qv::check_launch("kv8_attention");
 }
