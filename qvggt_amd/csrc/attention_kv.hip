@@ -46,6 +46,7 @@ struct KvAttn {
   int B, Lq, H, Hk, G, Lk, blocks, causal;
   int splits, split_tiles;   // splits of a sequence, key tiles of one: at least split_tiles
   int row_tiles;
+  uint32_t g_mul;         // floor(2^32 / G) + 1; 0 for G = 1
   long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;
   float scale_log2;
 };
@@ -145,19 +146,26 @@ struct KvRows {
   uint4 f[D / 16];
   float mul;
   __device__ __forceinline__ void load(const uint16_t* p, int h, float scale_log2) {
-    mul = scale_log2;
+    fetch(p, h);
+    finish(scale_log2);
+  }
+  __device__ __forceinline__ void fetch(const uint16_t* p, int h) {
 #pragma unroll
     for (int st = 0; st < D / 16; ++st)
       f[st] = *reinterpret_cast<const uint4*>(p + (KV8 ? 32 * (st >> 1) + 16 * h + 8 * (st & 1) : 16 * st + 8 * h));
+  }
+  __device__ __forceinline__ void finish(float scale_log2) {
+    mul = scale_log2;
     if constexpr (KV8 && BF16) {
-      float mx = 0.f;
+      u16x2 top = {0, 0};                      // magnitudes order like integers
 #pragma unroll
       for (int st = 0; st < D / 16; ++st) {
         const uint32_t w[4] = {f[st].x, f[st].y, f[st].z, f[st].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx = fmaxf(mx, fmaxf(__builtin_fabsf(to_f32((uint16_t)w[i], true)), __builtin_fabsf(to_f32((uint16_t)(w[i] >> 16), true))));
+        for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
       }
+      float mx = to_f32(top[0] > top[1] ? top[0] : top[1], true);
+      mx = mx < INFINITY ? mx : 1.0f;          // such a row comes to nothing anyway
       mx = kv_half_max(mx);
       int e = (int)(__builtin_bit_cast(uint32_t, mx) >> 23) - 127;
       e = e < -100 ? -100 : e;                 // the row's largest comes to 2^13 .. 2^14
@@ -343,6 +351,11 @@ struct KvSource {
   __device__ __forceinline__ void next() { at += step, left -= keys; }
 };
 
+// row / G: exact while row * G < 2^32
+__device__ __forceinline__ int kv_query(const KvAttn& a, int row) {
+  return a.g_mul ? (int)__umulhi((uint32_t)row, a.g_mul) : row;
+}
+
 __device__ __forceinline__ int kv_len(const KvAttn& a, int b) {
   if (!a.lens) return a.Lk;
   const int l = a.lens[b];
@@ -408,7 +421,7 @@ __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, f
                                          int h, bool live) {
   if (!live) return;
   const float inv = l == 0.f ? 0.f : __builtin_ldexpf(1.0f / l, ve);
-  const int qi = row / a.G, head = p.hk * a.G + row % a.G;
+  const int qi = kv_query(a, row), head = p.hk * a.G + row - qi * a.G;
   if (a.splits == 1) {
     uint16_t* op = a.out + p.b * a.o_bs + qi * a.o_ts + head * a.o_hs;
 #pragma unroll
@@ -513,11 +526,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int hk = part.hk, b = part.b;
   const int nrows = a.Lq * a.G;
   const int row0 = part.rt * ROWS;
-  const int first_query = row0 / a.G;
-  const KvRange rg = kv_range(a, b, part.split, first_query, (min(nrows, row0 + ROWS) - 1) / a.G);
+  const int first_query = kv_query(a, row0);
+  const KvRange rg = kv_range(a, b, part.split, first_query, kv_query(a, min(nrows, row0 + ROWS) - 1));
   if (first_query >= rg.nq) return;
   const int wrow = row0 + wave * 32, row = wrow + l32;
-  const bool live = wrow < nrows && wrow / a.G < rg.nq;      // wave-uniform
+  const bool live = wrow < nrows && kv_query(a, wrow) < rg.nq;      // wave-uniform
   const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
 
   TK kt;
@@ -573,7 +586,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     lds_barrier();
   };
   // tiles below edge are seen whole by all rows of the wave
-  const int wfirst = wrow / a.G;
+  const int wfirst = kv_query(a, wrow);
   const int edge = !KV8 && a.mask ? 0 : (a.causal ? min(rg.len, rg.len - rg.nq + wfirst + 1) : rg.len) / KV_BLOCK - rg.t0;
   auto visible = [&](int j) __attribute__((always_inline)) {
     uint64_t seen = ~0ull;
@@ -640,8 +653,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     KvRows<KV8, BF16, D> qr;
     const int rc = row < nrows ? row : nrows - 1;
-    const int qi = rc / a.G;
-    qr.load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc % a.G) * a.q_hs, h, a.scale_log2);
+    const int qi = kv_query(a, rc);
+    qr.load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h, a.scale_log2);
     const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;                      // the last key that the row sees
     auto frag_k = [&](int stage, int f) __attribute__((always_inline)) {               // f = kb + 2 st
       if constexpr (KV8) return reinterpret_cast<const uint4*>(k_lds[stage])[((f & 1) * KS + (f >> 1)) * 64 + lane];
@@ -722,7 +735,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   } else if (!live) {
     return;
   }
-  kv_store<BF16, D>(a, s, kv_half_sum(s.l), ve, part, row, h, row < nrows && row / a.G < rg.nq);
+  kv_store<BF16, D>(a, s, kv_half_sum(s.l), ve, part, row, h, row < nrows && kv_query(a, row) < rg.nq);
 }
 
 // ------------------------------------------------------------------ wide form
@@ -747,11 +760,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int hk = part.hk, b = part.b;
   const int nrows = a.Lq * a.G;
   const int row0 = part.rt * ROWS;
-  const int first_query = row0 / a.G;
-  const KvRange rg = kv_range(a, b, part.split, first_query, (min(nrows, row0 + ROWS) - 1) / a.G);
+  const int first_query = kv_query(a, row0);
+  const KvRange rg = kv_range(a, b, part.split, first_query, kv_query(a, min(nrows, row0 + ROWS) - 1));
   if (first_query >= rg.nq) return;
   const int wrow = row0 + wave * 32 * QB;
-  const bool live = wrow < nrows && wrow / a.G < rg.nq;      // wave-uniform
+  const bool live = wrow < nrows && kv_query(a, wrow) < rg.nq;      // wave-uniform
   const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
 
   TK kt;
@@ -791,7 +804,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   // tiles below edge are seen whole by all rows of the wave
   const int edge =
-      !KV8 && a.mask ? 0 : (a.causal ? min(rg.len, rg.len - rg.nq + wrow / a.G + 1) : rg.len) / KV_BLOCK - rg.t0;
+      !KV8 && a.mask ? 0 : (a.causal ? min(rg.len, rg.len - rg.nq + kv_query(a, wrow) + 1) : rg.len) / KV_BLOCK - rg.t0;
   // the keys of tile j that are there; value rows of the others may hold anything
   auto visible = [&](int j) __attribute__((always_inline)) {
     uint64_t seen = kv_below(rg.len - (rg.t0 + j) * KV_BLOCK);
@@ -832,8 +845,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = wrow + 32 * qb + l32, rc = r < nrows ? r : nrows - 1;
-    const int qi = rc / a.G;
-    qr[qb].load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc % a.G) * a.q_hs, h, a.scale_log2);
+    const int qi = kv_query(a, rc);
+    qr[qb].load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h, a.scale_log2);
     upto[qb] = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
     s[qb].init();
   }
@@ -892,21 +905,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = wrow + 32 * qb + l32;
-    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), ve, part, r, h, r < nrows && r / a.G < rg.nq);
+    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), ve, part, r, h, r < nrows && kv_query(a, r) < rg.nq);
   }
 }
 
 // ------------------------------------------------------------------ step form
+constexpr int kv_step_waves(bool kv8, int d) { return !kv8 && d == 64 ? 8 : 4; }
 template <bool KV8, bool BF16, int D>
 struct KvStep {
-  static constexpr int WAVES = 4;
-  static constexpr int KB = KV8 ? 2 : D == 64 ? 2 : 1;          // 32-key blocks of a tile
+  static constexpr int WAVES = kv_step_waves(KV8, D);
+  static constexpr int KB = KV8 ? 2 : 1;          // 32-key blocks of a tile
   static constexpr int KT = 32 * KB;
   static constexpr int TILE = KT * D * 2;
   static constexpr int LDS = KV8 ? WAVES * 32 * D * 4 : WAVES * 4 * TILE;   // the join's rows / 2 stages of K and V
 };
 template <bool KV8, bool BF16, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1, KV8 ? 2 : 1))) void kv_attn_step_kernel(const KvAttn a) {
+__global__ __launch_bounds__(64 * kv_step_waves(KV8, D)) __attribute__((amdgpu_waves_per_eu(KV8 || D == 64 ? 2 : 1, KV8 || D == 64 ? 2 : 1))) void kv_attn_step_kernel(const KvAttn a) {
   using C = KvStep<KV8, BF16, D>;
   constexpr bool MBF = BF16 && !KV8;
   constexpr int KS = D / 16, NV = D / 32, KB = C::KB, KT = C::KT, TILE = C::TILE;
@@ -915,39 +929,58 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
-  const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  // heads first: the first splits of a batch of different lengths are the full ones, and
+  // as the fastest index they would all lie on the same XCDs
+  const int hk = blockIdx.x, b = blockIdx.z, split = (blockIdx.y + blockIdx.z) % gridDim.y;
   const int nrows = a.Lq * a.G;                      // <= 32
   const KvRange rg = kv_range(a, b, split, 0, a.Lq - 1);
   if (rg.nq == 0) return;
+  const long record = (((long)b * a.splits + split) * a.Hk + hk) * nrows;     // of a split's first row
+  if (rg.t0 >= rg.t1 && a.splits > 1) {
+    if (tid < nrows) a.stat[record + tid] = make_float2(-INFINITY, 0.f);
+    return;
+  }
   const int rc = l32 < nrows ? l32 : nrows - 1;
-  const int qi = rc / a.G;
-  KvRows<KV8, BF16, D> qr;
-  qr.load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc % a.G) * a.q_hs, h, a.scale_log2);
+  const int qi = kv_query(a, rc);
+  const uint16_t* qp = a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs;
   const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
   const int first_upto = a.causal ? rg.len - rg.nq : rg.len - 1;
+  KvRows<KV8, BF16, D> qr;
   KvState<D> s;
   s.init();
   KvUnits units;
   int ve = 0;
   if constexpr (KV8) {
+    // fragments straight from memory: the next tile's K when this one's are used, its V
+    // behind the last product (no spare registers: a spilled one, read back behind these
+    // loads, would wait for them)
     const long cache0 = ((long)b * a.Hk + hk) * a.blocks;
     constexpr int U = KV_BLOCK * D / 1024;           // 1 KB pieces of a block's keys or values
     uint4 kraw[U], vraw[U];
     float ks = 0.f, vs = 0.f;
-    auto fetch = [&](int tile) __attribute__((always_inline)) {
+    auto fetch_k = [&](int tile) __attribute__((always_inline)) {
       const uint4* kp = reinterpret_cast<const uint4*>(a.kc) + (cache0 + tile) * (KV_BLOCK * D / 16) + lane;
-      const uint4* vp = reinterpret_cast<const uint4*>(a.vc) + (cache0 + tile) * (KV_BLOCK * D / 16) + lane;
 #pragma unroll
       for (int u = 0; u < U; ++u) kraw[u] = kp[64 * u];
+    };
+    auto fetch_v = [&](int tile) __attribute__((always_inline)) {
+      const uint4* vp = reinterpret_cast<const uint4*>(a.vc) + (cache0 + tile) * (KV_BLOCK * D / 16) + lane;
 #pragma unroll
       for (int u = 0; u < U; ++u) vraw[u] = vp[64 * u];
-      ks = a.ks[cache0 + tile];
-      vs = a.vs[cache0 + tile];
     };
+    qr.fetch(qp, h);                                 // before the tiles: loads come back in order
+    __builtin_amdgcn_sched_barrier(0);
     int tile = rg.t0 + wave;
-    if (tile < rg.t1) fetch(tile);
+    if (tile < rg.t1) {
+      fetch_k(tile);
+      ks = a.ks[cache0 + tile], vs = a.vs[cache0 + tile];
+      fetch_v(tile);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    qr.finish(a.scale_log2);
     for (; tile < rg.t1; tile += C::WAVES) {
       const int key0 = tile * KV_BLOCK;
+      const bool more = tile + C::WAVES < rg.t1;
       const uint64_t seen = kv_below(rg.len - key0);
       f32x16 sc[KB];
       uint4 pf[2 * KB], lo, hi;
@@ -961,25 +994,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
         }
       const float c = kv_factor((ks > 0.f || ks != ks ? ks : 1.0f) * qr.mul);
       const _Float16 f = (_Float16)units.fit(vs);
-      uint4 vnow[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) vnow[u] = vraw[u];
-      if (tile + C::WAVES < rg.t1) fetch(tile + C::WAVES);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) {
+        fetch_k(tile + C::WAVES);
+        ks = a.ks[cache0 + tile + C::WAVES], vs = a.vs[cache0 + tile + C::WAVES];
+      }
       if (units.ve != ve) {
         s.scale(__builtin_ldexpf(1.0f, ve - units.ve));
         ve = units.ve;
       }
-      if (seen != ~0ull || first_upto < key0 + KV_BLOCK - 1) 
-        kv_mask<KB>(sc, seen & kv_below(upto - key0 + 1), h);
+      if (seen != ~0ull || first_upto < key0 + KV_BLOCK - 1) kv_mask<KB>(sc, seen & kv_below(upto - key0 + 1), h);
       kv_softmax<MBF, D, KB, false>(sc, c, s, pf, [](int) __attribute__((always_inline)) {});
 #pragma unroll
       for (int db = 0; db < NV; ++db)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          kv_decode(vnow[db * 2 + w], (f16x2){f, f}, lo, hi);
+          kv_decode(vraw[db * 2 + w], (f16x2){f, f}, lo, hi);
           s.o[db] = kv_mfma<MBF>(lo, pf[2 * w], s.o[db]);
           s.o[db] = kv_mfma<MBF>(hi, pf[2 * w + 1], s.o[db]);
         }
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) fetch_v(tile + C::WAVES);
     }
   } else {
     // two stages of K and V in LDS for each wave, filled by its own copies
@@ -1008,10 +1043,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
       sk.next();
       sv.next();
     };
-    static_assert(2 * DMA == 16, "the wait below counts the copies of one stage");
+    static_assert(2 * DMA == 8 || 2 * DMA == 16, "the wait below counts the copies of one stage");
     int buf = 0;
     uint8_t mask_byte = 1;
+    qr.fetch(qp, h);
+    __builtin_amdgcn_sched_barrier(0);
     if (tile < t1) issue(0);
+    qr.finish(a.scale_log2);
     for (; tile < t1; tile += C::WAVES) {
       const int key0 = tile * KT;
       const bool more = tile + C::WAVES < t1;
@@ -1024,7 +1062,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the other stage's reads are done
       if (more) {
         issue(buf ^ 1);
-        asm volatile("s_waitcnt vmcnt(16)" ::: "memory");      // this stage's copies have landed
+        if constexpr (2 * DMA == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");      // this stage's copies have landed
+        else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
       } else {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       }
@@ -1077,8 +1116,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
             make_float4(s.o[db][4 * g] * by, s.o[db][4 * g + 1] * by, s.o[db][4 * g + 2] * by, s.o[db][4 * g + 3] * by);
   __syncthreads();
   const int rows_out = nrows < rg.nq * a.G ? nrows : rg.nq * a.G;
-  for (int i = tid; i < rows_out * (D / 4); i += 256) {
-    const int row = i / (D / 4), d = 4 * (i % (D / 4));
+  for (int i = tid; i < rows_out * (D / 4); i += 64 * C::WAVES) {
+    const int row = i / (D / 4), d = 4 * (i % (D / 4)), query = kv_query(a, row);
     float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int w = 0; w < C::WAVES; ++w) {
@@ -1086,14 +1125,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(KV8 ? 2 : 1
       o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
     }
     if (a.splits == 1) {
-      uint16_t* op = a.out + b * a.o_bs + (row / a.G) * a.o_ts + (hk * a.G + row % a.G) * a.o_hs + d;
+      uint16_t* op = a.out + b * a.o_bs + query * a.o_ts + (hk * a.G + row - query * a.G) * a.o_hs + d;
       *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF16>(o.x, o.y), pack2<BF16>(o.z, o.w));
     } else {
-      *reinterpret_cast<float4*>(a.part + ((((long)b * a.splits + split) * a.Hk + hk) * nrows + row) * D + d) = o;
+      *reinterpret_cast<float4*>(a.part + (record + row) * D + d) = o;
     }
   }
   if (a.splits > 1 && wave == 0 && h == 0 && l32 < rows_out) {
-    a.stat[(((long)b * a.splits + split) * a.Hk + hk) * nrows + l32] = make_float2(m, sum);
+    a.stat[record + l32] = make_float2(m, sum);
   }
 }
 
@@ -1107,7 +1146,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttn a) {
   const uint32_t row = i / (D / 4), per = (uint32_t)a.Lq * a.G;
   if (row >= per) return;
   const int d = 4 * (int)(i % (D / 4));
-  const int qi = row / a.G;
+  const int qi = kv_query(a, row);
   if (a.counts && qi >= a.counts[b]) return;
   const long rows = (long)a.Hk * per;                // of a split
   const long at = (long)b * a.splits * rows + (long)hk * per + row;
@@ -1128,7 +1167,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttn a) {
     o.z = o.z * keep + (w != 0.f ? w * x.z : 0.f), o.w = o.w * keep + (w != 0.f ? w * x.w : 0.f);
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  uint16_t* op = a.out + b * a.o_bs + qi * a.o_ts + (hk * a.G + (int)row % a.G) * a.o_hs + d;
+  uint16_t* op = a.out + b * a.o_bs + qi * a.o_ts + (hk * a.G + (int)row - qi * a.G) * a.o_hs + d;
   *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
 }
 
@@ -1144,9 +1183,13 @@ static KvPlan kv_plan(bool kv8, int64_t B, int64_t Lq, int64_t H, int64_t Hk, in
   KvPlan p = {};
   if (rows <= 32) {
     p.step = true, p.qb = 1, p.row_tiles = 1;
-    const int64_t slots = kv8 ? 512 : 256;
+    // 8-bit: two workgroups a CU, twice as many splits where sequences may differ (16 of up
+    // to 8001 tokens: as fast when all are full, 19 instead of 27 us when all hold 2048).
+    // 16-bit: one a CU, and from half the CUs on no split, which saves the join (8 x 16 heads
+    // over 1374 keys: 11.3 us; split in two 12.3 and 3.9)
+    const int64_t slots = kv8 ? (B > 1 ? 1024 : 512) : heads >= 128 ? 1 : 256;
     int64_t s = heads < slots ? slots / (heads > 0 ? heads : 1) : 1;
-    if (s > tiles / 8) s = tiles / 8;                       // two tiles a wave at least
+    if (s > tiles / 8) s = tiles / 8;                       // a tile or two for each wave at least
     if (s > 64) s = 64;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
@@ -1182,7 +1225,7 @@ static void kv_launch(const KvAttn& a, const KvPlan& p, hipStream_t st) {
   const int64_t n = (int64_t)a.B * a.Hk * p.splits * p.row_tiles, round = 8 * KV_NEAR;
   const unsigned wg = (unsigned)((n + round - 1) / round * round);
   if (p.step) {
-    hipLaunchKernelGGL((kv_attn_step_kernel<KV8, BF16, D>), dim3(p.splits, a.Hk, a.B), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv_attn_step_kernel<KV8, BF16, D>), dim3(a.Hk, p.splits, a.B), dim3(64 * kv_step_waves(KV8, D)), 0, st, a);
   } else if (D == 64 && p.qb == 2) {
     hipLaunchKernelGGL((kv_attn_wide_kernel<KV8, BF16>), dim3(wg), dim3(256), 0, st, a);
   } else {
@@ -1204,7 +1247,8 @@ static int kv_common(KvAttn& a, const char* what, const void* q, void* out, int 
                "bad shape B=%lld Lq=%lld Lk=%lld heads=%lld / %lld", (long long)B, (long long)Lq, (long long)Lk,
                (long long)H, (long long)Hk);
   QV_CHECK_ARG(scale > 0.f && scale < INFINITY, "the scale must be a positive number");
-  QV_CHECK_ARG(Lq * (H / Hk) <= INT32_MAX / 2 && B * H * Lq <= (1ll << 36), "too many rows");
+  QV_CHECK_ARG(Lq * (H / Hk) <= INT32_MAX / 2 && Lq * (H / Hk) * (H / Hk) < (1ll << 32) && B * H * Lq <= (1ll << 36),
+               "too many rows");
   if (B == 0 || Lq == 0) return QV_OK;
   QV_CHECK_ARG(q && out && qs && os, "null pointer argument");
   QV_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0, "q must be 16-byte and out 8-byte aligned");
@@ -1214,6 +1258,7 @@ static int kv_common(KvAttn& a, const char* what, const void* q, void* out, int 
   a.B = (int)B, a.Lq = (int)Lq, a.Lk = (int)Lk, a.H = (int)H, a.Hk = (int)Hk, a.G = (int)(H / Hk);
   a.q_bs = qs[0], a.q_ts = qs[1], a.q_hs = qs[2];
   a.o_bs = os[0], a.o_ts = os[1], a.o_hs = os[2];
+  a.g_mul = a.G == 1 ? 0 : (uint32_t)((1ull << 32) / a.G + 1);
   a.scale_log2 = scale * 1.4426950408889634f;
   return QV_OK;
 }
