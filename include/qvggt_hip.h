@@ -354,13 +354,14 @@ int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* positions,
  * and head strides in elements, multiples of 8; dims contiguous.
  * Sequence b gets its first counts[b] tokens (NULL: n) behind start[b] cached ones
  * (what it held behind them is dropped, what does not fit is left out), and lens[b] is
- * set to their number; start may be lens itself.  tickets: B words, 0 at the first
- * call, kept with the cache.  A block's scale is the smallest number of four
+ * set to their number; start may be lens itself.  tickets: B * (Hk + 1) *
+ * QV_KV8_TICKETS words, 0 at the first call, kept with the cache.  A block's scale is the smallest number of four
  * significant bits that is at least amax / 127 over its new tokens, or the one it had
  * where that is larger; value = code * scale, code = rint(x / scale), ties to even; the
  * old codes of a block whose scale grows are rounded again.  A NaN or infinity
  * makes the scale NaN until the block is begun again.
  */
+#define QV_KV8_TICKETS 32
 int qv_kv8_append(const void* k, const void* v, int dtype, void* k_codes, void* v_codes,
                   float* k_scales, float* v_scales, const int32_t* start, int32_t* lens,
                   uint32_t* tickets, const int32_t* counts, int64_t B, int64_t n, int64_t Hk,

@@ -21,6 +21,7 @@ QV_EPI_BIAS_GELU = 2
 QV_EPI_GELU = 3
 QV_ROPE_BLOCK = 0
 QV_ROPE_HALF = 1
+QV_KV8_TICKETS = 32
 
 _vp = C.c_void_p
 _i64 = C.c_int64

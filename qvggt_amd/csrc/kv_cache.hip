@@ -18,6 +18,8 @@
 
 namespace qv {
 
+constexpr int KV_TICKET = QV_KV8_TICKETS;   // words from ticket to ticket
+
 // The smallest number of four significant bits that is at least amax / 127, not
 // below 2^-120 (so that its reciprocal and every border stay normal numbers); 0
 // for 0.  c has the right exponent and its first three fraction bits cut off
@@ -40,6 +42,11 @@ __device__ __forceinline__ int kv_code(float x, float s, float inv) {
   return x < 0.f ? -c : c;
 }
 
+// Where byte `off` of a block lies while it is put together or taken apart in LDS: 16
+// bytes more after every 4 units and after every 32.  Rows of keys (units 32 apart) and
+// of values (units 8 apart) would otherwise meet the same banks, 8 to 16 lanes at once.
+__host__ __device__ __forceinline__ constexpr int kv_skew(int off) { return off + ((off >> 6) + (off >> 9)) * 16; }
+
 // One workgroup per block that the call touches and key head: D * 2 threads for the
 // keys, as many for the values; a thread takes 4 consecutive tokens of 8 dims, one
 // dword of a value unit for each dim and 8 bytes of a key unit for each token.
@@ -53,7 +60,8 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
     int blocks, long k_bs, long k_ts, long k_hs, long v_bs, long v_ts, long v_hs) {
   constexpr int BYTES = KV_BLOCK * D;      // of one block's keys or values
   constexpr int HALF = 2 * D;              // threads for each of the two
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BYTES];
+  constexpr int STAGE = kv_skew(BYTES);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
   __shared__ uint32_t wave_max[4 * D / 64];
   const int tid = threadIdx.x;
   const bool val = tid >= HALF;            // wave-uniform
@@ -115,8 +123,8 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
     const bool grown = old && s > was;
     const bool whole = !old || grown;      // the same for all threads of a half
     const float inv = s > 0.f ? 1.0f / s : 0.f;
-    uint8_t* stage = lds + (val ? BYTES : 0);
-    if (whole) {
+    uint8_t* stage = lds + (val ? STAGE : 0);
+    if (whole && (grown || end < KV_BLOCK)) {
       // the old codes, rounded to the new scale, zero behind them
       for (int i = t; i < BYTES / 16; i += HALF) {
         uint4 u = make_uint4(0, 0, 0, 0);
@@ -135,7 +143,7 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
           }
           u = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        reinterpret_cast<uint4*>(stage)[i] = u;
+        *reinterpret_cast<uint4*>(stage + kv_skew(16 * i)) = u;
       }
     }
     __syncthreads();                       // also: every thread has read the old scale
@@ -153,19 +161,19 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
         }
       }
     }
-    uint8_t* to = whole ? stage : codes;
+    auto at = [&](int off) __attribute__((always_inline)) { return whole ? stage + kv_skew(off) : codes + off; };
     if (!val) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (tok + r >= old && tok + r < end)
-          *reinterpret_cast<uint2*>(to + kv_key_offset<D>(tok + r, 8 * g)) = make_uint2(c[r][0], c[r][1]);
+          *reinterpret_cast<uint2*>(at(kv_key_offset<D>(tok + r, 8 * g))) = make_uint2(c[r][0], c[r][1]);
     } else if (tok >= old && tok + 4 <= end) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {        // token 4i is on a dword
         uint32_t w = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) w |= ((c[r][e >> 2] >> (8 * (e & 3))) & 0xFF) << (8 * r);
-        *reinterpret_cast<uint32_t*>(to + kv_value_offset<D>(tok, 8 * g + e)) = w;
+        *reinterpret_cast<uint32_t*>(at(kv_value_offset<D>(tok, 8 * g + e))) = w;
       }
     } else {
 #pragma unroll
@@ -173,18 +181,25 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
         if (tok + r >= old && tok + r < end)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            to[kv_value_offset<D>(tok + r, 8 * g + e)] = (uint8_t)(c[r][e >> 2] >> (8 * (e & 3)));
+            *at(kv_value_offset<D>(tok + r, 8 * g + e)) = (uint8_t)(c[r][e >> 2] >> (8 * (e & 3)));
     }
     __syncthreads();
     if (whole)
       for (int i = t; i < BYTES / 16; i += HALF)
-        reinterpret_cast<uint4*>(codes)[i] = reinterpret_cast<const uint4*>(stage)[i];
+        reinterpret_cast<uint4*>(codes)[i] = *reinterpret_cast<const uint4*>(stage + kv_skew(16 * i));
   }
-  // start and lens may be one tensor: the length is written by the last workgroup of
-  // the sequence, when all have read the start.  The ticket wraps to 0 by itself.
+  // The length is written when all workgroups of the sequence have read the start, if that
+  // is the same tensor: by the last one, found by tickets that wrap to 0 by themselves (one
+  // for each head and one for the heads, on lines of their own: 376 increments of a
+  // sequence's one word took longer than the codes).
   if (tid == 0) {
-    const uint32_t last = gridDim.x * gridDim.y - 1;
-    if (atomicInc(tickets + b, last) == last) lens_out[b] = start + cnt;
+    bool last = head == 0 && blockIdx.x == 0;
+    if (start_in == lens_out) {
+      uint32_t* mine = tickets + (size_t)b * (Hk + 1) * KV_TICKET;
+      last = gridDim.x == 1 || atomicInc(mine + (head + 1) * KV_TICKET, gridDim.x - 1) == gridDim.x - 1;
+      if (last) last = atomicInc(mine, (uint32_t)Hk - 1) == (uint32_t)Hk - 1;
+    }
+    if (last) lens_out[b] = start + cnt;
   }
 }
 
@@ -197,7 +212,7 @@ __global__ __launch_bounds__(256) void kv8_values_kernel(
     int Hk, int blocks, uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out) {
   constexpr int BYTES = KV_BLOCK * D;
   constexpr int ES = DT == QV_F32 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kv_skew(BYTES)];
   const int tid = threadIdx.x, head = blockIdx.y;
   const bool val = blockIdx.z & 1;
   const int b = blockIdx.z >> 1;
@@ -215,25 +230,34 @@ __global__ __launch_bounds__(256) void kv8_values_kernel(
   float s = 0.f;
   if (lo < len) {
     const uint4* from = reinterpret_cast<const uint4*>((val ? v_codes : k_codes) + which * BYTES);
-    for (int i = tid; i < BYTES / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = from[i];
+    for (int i = tid; i < BYTES / 16; i += 256) *reinterpret_cast<uint4*>(lds + kv_skew(16 * i)) = from[i];
     s = (val ? v_scales : k_scales)[which];
   }
   __syncthreads();
   uint8_t* out = val ? v_out : k_out;
-  for (int i = tid; i < (hi - lo) * (D / 4); i += 256) {     // 4 dims of one token
-    const int p = lo + i / (D / 4), d = 4 * (i % (D / 4));
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p < len) {
-      const int tok = p - block * KV_BLOCK;
+  // a thread takes 4 dims of 4 consecutive tokens: a dword of codes for each of the tokens
+  // (keys) or dims (values)
+  for (int i = tid; i < KV_BLOCK / 4 * (D / 4); i += 256) {
+    const int tok = 4 * (i / (D / 4)), d = 4 * (i % (D / 4)), p0 = block * KV_BLOCK + tok;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = *reinterpret_cast<const uint32_t*>(
+          lds + kv_skew(val ? kv_value_offset<D>(tok, d + e) : kv_key_offset<D>(tok + e, d)));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = p0 + r;
+      if (p < lo || p >= hi) continue;
+      float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        x[e] = s * (float)(int8_t)lds[val ? kv_value_offset<D>(tok, d + e) : kv_key_offset<D>(tok, d + e)];
-    }
-    uint8_t* to = out + ((((long)b * n + (p - first)) * Hk + head) * D + d) * ES;
-    if constexpr (DT == QV_F32) {
-      *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack2<DT == QV_BF16>(x[0], x[1]), pack2<DT == QV_BF16>(x[2], x[3]));
+        x[e] = p < len ? s * (float)(int8_t)(val ? w[e] >> (8 * r) : w[r] >> (8 * e)) : 0.f;
+      uint8_t* to = out + ((((long)b * n + (p - first)) * Hk + head) * D + d) * ES;
+      if constexpr (DT == QV_F32) {
+        *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<DT == QV_BF16>(x[0], x[1]), pack2<DT == QV_BF16>(x[2], x[3]));
+      }
     }
   }
 }

@@ -50,7 +50,7 @@ class Int8KVCache:
         self.k_scales = torch.zeros(shape[:3], dtype=torch.float32, **kw)
         self.v_scales = torch.zeros(shape[:3], dtype=torch.float32, **kw)
         self.lens = torch.zeros(batch, dtype=torch.int32, **kw)
-        self._tickets = torch.zeros(batch, dtype=torch.int32, **kw)
+        self._tickets = torch.zeros(batch * (kv_heads + 1) * _lib.QV_KV8_TICKETS, dtype=torch.int32, **kw)
         self._bound = 0
 
     # ------------------------------------------------------------- contents
