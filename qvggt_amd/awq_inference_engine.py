@@ -825,7 +825,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, plan: RopeAxesPlan, out:
     if T == 0 or H == 0:
         return out
     pos = _contig(positions)
-    sections = (C.c_int64 * axes)(*plan.sections)
+    sections = _i64s(*plan.sections)
     layout = _lib.QV_ROPE_BLOCK if plan.layout == "block" else _lib.QV_ROPE_HALF
     with _device(dev):
         _lib.call("qv_rope_axes", _ptr(x), _ptr(out), dt, _ptr(pos), _ptr(plan.turns), sections, axes, layout, T, H, D,
@@ -876,9 +876,17 @@ def _kv_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+@functools.lru_cache(maxsize=4096)
+def _i64s(*values: int):
+    """A C array of these numbers (only read by the library, so one serves all calls)."""
+    return (C.c_int64 * len(values))(*values)
+
+
 def _kv_strides(t: torch.Tensor):
     """Batch, token and head strides; 0 for a dim of one."""
-    return (C.c_int64 * 3)(*(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+    B, n, H, _ = t.shape
+    sb, st, sh, _ = t.stride()
+    return _i64s(sb if B != 1 else 0, st if n != 1 else 0, sh if H != 1 else 0)
 
 
 @functools.lru_cache(maxsize=1024)

@@ -40,30 +40,30 @@ struct RopePiece {
   __device__ __forceinline__ void load(const uint8_t* p) {
     if constexpr (BYTES == 2) {
       w[0] = *reinterpret_cast<const uint16_t*>(p);
-    } else if constexpr (BYTES == 4) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else if constexpr (BYTES == 8) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      w[0] = u.x, w[1] = u.y;
     } else {
+      constexpr int N = BYTES >= 16 ? 4 : BYTES / 4;
+      typedef uint32_t vec __attribute__((ext_vector_type(N)));
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) {
-        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+      for (int i = 0; i < WORDS / N; ++i) {
+        const vec u = reinterpret_cast<const vec*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[N * i + j] = u[j];
       }
     }
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
     if constexpr (BYTES == 2) {
       *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
-    } else if constexpr (BYTES == 4) {
-      *reinterpret_cast<uint32_t*>(p) = w[0];
-    } else if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     } else {
+      constexpr int N = BYTES >= 16 ? 4 : BYTES / 4;
+      typedef uint32_t vec __attribute__((ext_vector_type(N)));
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i)
-        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      for (int i = 0; i < WORDS / N; ++i) {
+        vec u;
+#pragma unroll
+        for (int j = 0; j < N; ++j) u[j] = w[N * i + j];
+        reinterpret_cast<vec*>(p)[i] = u;
+      }
     }
   }
   __device__ __forceinline__ float get(int i) const {
@@ -82,46 +82,47 @@ struct RopePiece {
 };
 
 // token tile TB: TB * pairs table entries (at most ROPE_TABLE) and TB * H * groups
-// pieces of x, taken ROPE_UNITS a thread at a time.
+// pieces of x, taken ROPE_UNITS a thread at a time.  per_tok_mul, groups_mul:
+// floor(2^32 / n) + 1 for the pieces of a token and of a head (0: one token, one piece),
+// which divide exactly while the dividend times n is below 2^32.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void rope_axes_kernel(
     const uint8_t* x, uint8_t* out, const int32_t* __restrict__ pos, int axes, const double* __restrict__ turns, RopeAxes ra,
-    long T, int H, int pairs, int TB, long x_ts, long x_hs, long o_ts, long o_hs) {   // x and out may be the same
+    long T, int H, int pairs, int TB, uint32_t per_tok_mul, uint32_t groups_mul, long x_ts, long x_hs, long o_ts,
+    long o_hs) {   // x and out may be the same
   __shared__ float2 table[ROPE_TABLE];
   const int tid = threadIdx.x;
   const long tok0 = (long)blockIdx.x * TB;
   const int ntok = (int)(T - tok0 < TB ? T - tok0 : TB);
   const int groups = pairs / V, per_tok = H * groups, units = ntok * per_tok;
   constexpr int ES = RopePiece<DT, V>::ES;
+  x += tok0 * x_ts * ES;
+  out += tok0 * o_ts * ES;
 
   RopePiece<DT, V> lo[ROPE_UNITS], hi[ROPE_UNITS];
-  // where piece u lies: its token in the tile, its byte offsets in x and out, its first pair
-  auto locate = [&](int u, int& tok, int& pair, long& xo, long& oo, int& gap, bool& turn) {
-    tok = u / per_tok;
-    const int rest = u - tok * per_tok;
-    const int head = rest / groups;
-    pair = (rest - head * groups) * V;
-    int lo0 = ra.lo0[0], p0 = 0, ax = ra.axis[0];
-    gap = ra.gap[0];
-#pragma unroll
-    for (int c = 1; c < 5; ++c)
-      if (c < ra.chunks && pair >= ra.pair0[c]) lo0 = ra.lo0[c], p0 = ra.pair0[c], gap = ra.gap[c], ax = ra.axis[c];
-    const int dim = lo0 + pair - p0;
-    turn = ax >= 0;
-    xo = ((tok0 + tok) * x_ts + head * x_hs + dim) * ES;
-    oo = ((tok0 + tok) * o_ts + head * o_hs + dim) * ES;
-  };
-  auto fetch = [&](int base) {
+  int entry[ROPE_UNITS];                             // of the table; -1: copied
+  int gap[ROPE_UNITS];                               // bytes from lo to hi
+  long to[ROPE_UNITS];                               // byte offset in out
+  // pieces base .. base + 1023: where they lie (token, head, pairs), and their loads
+  auto fetch = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < ROPE_UNITS; ++i) {
       const int u = base + 256 * i + tid;
       if (u < units) {
-        int tok, pair, gap;
-        bool turn;
-        long xo, oo;
-        locate(u, tok, pair, xo, oo, gap, turn);
-        lo[i].load(x + xo);
-        hi[i].load(x + xo + (long)gap * ES);
+        const int tok = per_tok_mul ? (int)__umulhi((uint32_t)u, per_tok_mul) : 0;
+        const int rest = u - tok * per_tok;
+        const int head = groups_mul ? (int)__umulhi((uint32_t)rest, groups_mul) : rest;
+        const int pair = (rest - head * groups) * V;
+        int dim = ra.lo0[0] + pair, ax = ra.axis[0], g = ra.gap[0];
+#pragma unroll
+        for (int c = 1; c < 5; ++c)
+          if (c < ra.chunks && pair >= ra.pair0[c]) dim = ra.lo0[c] + pair - ra.pair0[c], g = ra.gap[c], ax = ra.axis[c];
+        entry[i] = ax < 0 ? -1 : tok * pairs + pair;
+        gap[i] = g * ES;
+        to[i] = (tok * o_ts + head * o_hs + dim) * ES;
+        const uint8_t* from = x + (tok * x_ts + head * x_hs + dim) * ES;
+        lo[i].load(from);
+        hi[i].load(from + gap[i]);
       }
     }
   };
@@ -144,27 +145,107 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(
     if (base) fetch(base);
 #pragma unroll
     for (int i = 0; i < ROPE_UNITS; ++i) {
-      const int u = base + 256 * i + tid;
-      if (u < units) {
-        int tok, pair, gap;
-        bool turn;
-        long xo, oo;
-        locate(u, tok, pair, xo, oo, gap, turn);
-        if (turn) {
-          RopePiece<DT, V> a, b;
+      if (base + 256 * i + tid < units) {
+        RopePiece<DT, V> a = lo[i], b = hi[i];
+        if (entry[i] >= 0) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float2 cs = table[tok * pairs + pair + e];
+            const float2 cs = table[entry[i] + e];
             const float l = lo[i].get(e), h = hi[i].get(e);
             a.set(e, __builtin_fmaf(l, cs.x, -(h * cs.y)));
             b.set(e, __builtin_fmaf(h, cs.x, l * cs.y));
           }
-          a.store(out + oo);
-          b.store(out + oo + (long)gap * ES);
-        } else {
-          lo[i].store(out + oo);
-          hi[i].store(out + oo + (long)gap * ES);
         }
+        a.store(out + to[i]);
+        b.store(out + to[i] + gap[i]);
+      }
+    }
+  }
+}
+
+// The same for heads of 64 to 512 dims (a power of two) with chunks in multiples of 4: a
+// lane takes 8 consecutive dims, so that rows are read and written whole, and reads the
+// partners of each 4 of them a second time (from the L1).  A row lies within one wave,
+// whose loads all come before its stores: x and out may be the same.  43968 tokens of 32
+// heads of 64 fp16 dims (16 + 24 + 24 by axis): 64 us, 5.6 TB/s.
+template <int DT>
+__global__ __launch_bounds__(256) void rope_axes_rows_kernel(
+    const uint8_t* x, uint8_t* out, const int32_t* __restrict__ pos, int axes, const double* __restrict__ turns, RopeAxes ra,
+    long T, int H, int pairs, int TB, uint32_t h_mul, long x_ts, long x_hs, long o_ts, long o_hs) {
+  __shared__ __attribute__((aligned(16))) float2 table[ROPE_TABLE];
+  constexpr int ES = RopePiece<DT, 4>::ES;
+  const int tid = threadIdx.x;
+  const long tok0 = (long)blockIdx.x * TB;
+  const int ntok = (int)(T - tok0 < TB ? T - tok0 : TB);
+  const int lanes = pairs / 4;                       // of a row
+  const int rows = ntok * H, step = 256 / lanes;
+  const int dim0 = tid % lanes * 8;
+  // this lane's two 4-dim pieces: their first pair (-1: copied), partner and sign
+  int entry[2], part[2];
+  float sign[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = dim0 + 4 * k;
+    entry[k] = -1, part[k] = d, sign[k] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 5; ++c)
+      if (c < ra.chunks && ra.axis[c] >= 0) {
+        const int len = ra.pair0[c + 1] - ra.pair0[c], lo = d - ra.lo0[c], hi = lo - ra.gap[c];
+        if (lo >= 0 && lo < len) entry[k] = ra.pair0[c] + lo, part[k] = d + ra.gap[c], sign[k] = -1.f;
+        if (hi >= 0 && hi < len) entry[k] = ra.pair0[c] + hi, part[k] = d - ra.gap[c], sign[k] = 1.f;
+      }
+  }
+  x += tok0 * x_ts * ES;
+  out += tok0 * o_ts * ES;
+  RopePiece<DT, 8> own[ROPE_UNITS];
+  RopePiece<DT, 4> other[ROPE_UNITS][2];
+  auto fetch = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int row = base + step * i + tid / lanes;
+      if (row < rows) {
+        const int tok = h_mul ? (int)__umulhi((uint32_t)row, h_mul) : row;
+        const uint8_t* from = x + (tok * x_ts + (row - tok * H) * x_hs) * ES;
+        own[i].load(from + dim0 * ES);
+        other[i][0].load(from + part[0] * ES);
+        other[i][1].load(from + part[1] * ES);
+      }
+    }
+  };
+  fetch(0);
+  for (int e = tid; e < ntok * pairs; e += 256) {
+    const int tok = e / pairs, pair = e - tok * pairs;
+    int ax = ra.axis[0];
+#pragma unroll
+    for (int c = 1; c < 5; ++c)
+      if (c < ra.chunks && pair >= ra.pair0[c]) ax = ra.axis[c];
+    float s = 0.f, c = 1.f;
+    if (ax >= 0) {
+      const double t = (double)pos[(tok0 + tok) * axes + ax] * turns[pair];
+      sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    }
+    table[e] = make_float2(c, s);
+  }
+  __syncthreads();
+  for (int base = 0; base < rows; base += step * ROPE_UNITS) {
+    if (base) fetch(base);
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int row = base + step * i + tid / lanes;
+      if (row < rows) {
+        const int tok = h_mul ? (int)__umulhi((uint32_t)row, h_mul) : row;
+        RopePiece<DT, 8> r = own[i];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (entry[k] >= 0) {
+            const float2* t = table + tok * pairs + entry[k];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 cs = t[e];
+              r.set(4 * k + e, __builtin_fmaf(own[i].get(4 * k + e), cs.x, sign[k] * (other[i][k].get(e) * cs.y)));
+            }
+          }
+        r.store(out + (tok * o_ts + (row - tok * H) * o_hs + dim0) * ES);
       }
     }
   }
@@ -172,12 +253,15 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(
 
 template <int DT>
 static void rope_axes_launch(int vec, unsigned grid, hipStream_t st, const void* x, void* out, const int32_t* pos, int axes,
-                             const double* turns, const RopeAxes& ra, long T, int H, int pairs, int TB, long x_ts,
-                             long x_hs, long o_ts, long o_hs) {
+                             const double* turns, const RopeAxes& ra, long T, int H, int pairs, int TB,
+                             uint32_t per_tok_mul, uint32_t mul, long x_ts, long x_hs, long o_ts, long o_hs) {
 #define QV_ROPE(V)                                                                                                   \
   hipLaunchKernelGGL((rope_axes_kernel<DT, V>), dim3(grid), dim3(256), 0, st, (const uint8_t*)x, (uint8_t*)out, pos, \
-                     axes, turns, ra, T, H, pairs, TB, x_ts, x_hs, o_ts, o_hs)
-  if (vec == 8) QV_ROPE(8);
+                     axes, turns, ra, T, H, pairs, TB, per_tok_mul, mul, x_ts, x_hs, o_ts, o_hs)
+  if (vec == 0)
+    hipLaunchKernelGGL((rope_axes_rows_kernel<DT>), dim3(grid), dim3(256), 0, st, (const uint8_t*)x, (uint8_t*)out, pos, axes,
+                       turns, ra, T, H, pairs, TB, mul, x_ts, x_hs, o_ts, o_hs);
+  else if (vec == 8) QV_ROPE(8);
   else if (vec == 4) QV_ROPE(4);
   else if (vec == 2) QV_ROPE(2);
   else QV_ROPE(1);
@@ -193,7 +277,7 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   QV_CHECK_ARG(dtype == QV_F16 || dtype == QV_BF16 || dtype == QV_F32, "bad dtype %d", dtype);
   QV_CHECK_ARG(axes >= 1 && axes <= 4, "1 to 4 axes are supported (got %lld)", (long long)axes);
   QV_CHECK_ARG(layout == QV_ROPE_BLOCK || layout == QV_ROPE_HALF, "bad layout %d", layout);
-  QV_CHECK_ARG(T >= 0 && H > 0 && D > 0 && D % 2 == 0 && D <= 1024 && H <= 65536, "bad shape T=%lld H=%lld D=%lld",
+  QV_CHECK_ARG(T >= 0 && H > 0 && D > 0 && D % 2 == 0 && D <= 1024 && H <= 4096, "bad shape T=%lld H=%lld D=%lld",
                (long long)T, (long long)H, (long long)D);
   QV_CHECK_ARG(sections, "null sections");
   qv::RopeAxes ra = {};
@@ -237,18 +321,28 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   }
   QV_CHECK_ARG((uintptr_t)x % es == 0 && (uintptr_t)out % es == 0, "x and out must be aligned to their type");
   const int pairs = (int)(D / 2);
-  const int64_t per_tok = H * (pairs / vec);
-  // tokens of a workgroup: one piece round (1024 pieces), at most the table, and
+  // whole rows: 8 dims a lane, rows within a wave, chunks in fours, and enough of them that
+  // bytes count (T x 32 heads of 64 fp16 dims: 43968 tokens 64 us, in pieces 70; 1374
+  // tokens 6.4 and 5.2)
+  const int wide = 8 * es < 16 ? 8 * es : 16;
+  const bool rows = 2 * T * H * D * es > (64 << 20) && vec >= 4 && D >= 64 && D <= 512 && (D & (D - 1)) == 0 && x_token_stride % 8 == 0 &&
+                    x_head_stride % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0 &&
+                    (uintptr_t)x % wide == 0 && (uintptr_t)out % wide == 0;
+  const int64_t per_tok = rows ? H * (D / 8) : H * (pairs / vec);
+  // tokens of a workgroup: one round of pieces (1024), at most the table, and
   // enough workgroups to fill the chip
   int64_t tb = 256 * qv::ROPE_UNITS / per_tok;
   if (tb > qv::ROPE_TABLE / pairs) tb = qv::ROPE_TABLE / pairs;
   if (tb > T / 1024) tb = T / 1024;
   if (tb < 1) tb = 1;
   const int64_t grid = (T + tb - 1) / tb;
+  const auto mul = [](int64_t n) { return n == 1 ? 0u : (uint32_t)((1ull << 32) / n + 1); };
+  const uint32_t per_tok_mul = tb == 1 ? 0u : mul(per_tok), second = rows ? mul(H) : mul(pairs / vec);
+  if (rows) vec = 0;
   QV_CHECK_ARG(grid <= INT32_MAX && per_tok * tb <= INT32_MAX / 2, "too many tokens or heads");
 #define QV_ARGS                                                                                                       \
   vec, (unsigned)grid, (hipStream_t)stream, x, out, positions, (int)axes, turns, ra, (long)T, (int)H, pairs, (int)tb, \
-      (long)x_token_stride, (long)x_head_stride, (long)out_token_stride, (long)out_head_stride
+      per_tok_mul, second, (long)x_token_stride, (long)x_head_stride, (long)out_token_stride, (long)out_head_stride
   if (dtype == QV_F16) qv::rope_axes_launch<QV_F16>(QV_ARGS);
   else if (dtype == QV_BF16) qv::rope_axes_launch<QV_BF16>(QV_ARGS);
   else qv::rope_axes_launch<QV_F32>(QV_ARGS);
