@@ -145,10 +145,6 @@ struct KvRows {
   static constexpr bool MBF = BF16 && !KV8;   // MFMA type
   uint4 f[D / 16];
   float mul;
-  __device__ __forceinline__ void load(const uint16_t* p, int h, float scale_log2) {
-    fetch(p, h);
-    finish(scale_log2);
-  }
   __device__ __forceinline__ void fetch(const uint16_t* p, int h) {
 #pragma unroll
     for (int st = 0; st < D / 16; ++st)
@@ -457,7 +453,7 @@ struct KvTiles {
   static constexpr int RPD = 1024 / (2 * D);         // rows of a copy
   static constexpr int UNITS = KV_BLOCK * D / 16 / 256;   // 16-byte units of a thread
   KvSource src;
-  uint32_t voff[DMA];
+  uint32_t row_off, chunk;                           // of the lane in a copy: its row, its swizzled 16 bytes
   const uint4* codes;
   __device__ __forceinline__ void init(const KvAttn& a, int b, int hk, const KvRange& rg, int wave, int lane) {
     if constexpr (KV8) {
@@ -466,11 +462,11 @@ struct KvTiles {
     } else {
       if constexpr (V) src.init(a.v + b * a.v_bs + hk * a.v_hs, a.v_ts, D, rg.len, (int64_t)rg.t0 * KV_BLOCK, KV_BLOCK);
       else src.init(a.k + b * a.k_bs + hk * a.k_hs, a.k_ts, D, rg.len, (int64_t)rg.t0 * KV_BLOCK, KV_BLOCK);
-#pragma unroll
-      for (int w = 0; w < DMA; ++w) {
-        const int r = RPD * (DMA * wave + w) + lane / (D / 8), c = lane % (D / 8);
-        voff[w] = (uint32_t)(lane / (D / 8)) * src.row + ((c ^ (V ? kv_fv<D>(r) : kv_fk<D>(r))) * 16);
-      }
+      // copy w of a wave holds rows RPD (DMA wave + w) ..: the swizzle of V depends on the lane
+      // only, that of K flips with w
+      const int r = lane / (D / 8), c = lane % (D / 8);
+      row_off = (uint32_t)r * src.row;
+      chunk = (uint32_t)(c ^ (V ? kv_fv<D>(r) : kv_fk<D>(r))) * 16;
     }
   }
   // the next tile on its way to LDS (16-bit) or registers
@@ -484,7 +480,7 @@ struct KvTiles {
 #pragma unroll
       for (int w = 0; w < DMA; ++w) {
         const int r0 = RPD * (DMA * wave + w);
-        kv_dma16(r, voff[w], (uint32_t)r0 * src.row, lds + r0 * (2 * D));
+        kv_dma16(r, row_off + (V ? chunk : chunk ^ (w * (D == 64 ? 16u : 64u))), (uint32_t)r0 * src.row, lds + r0 * (2 * D));
       }
       src.next();
     }
@@ -505,19 +501,16 @@ struct KvTiles {
 // 4 waves of 32 rows.  Beside tile j's softmax run the QK of tile j + 1 and the PV of tile
 // j - 1, a few of each in every slot, so that no product stands alone.  K is in LDS two
 // tiles ahead, V comes with its own tile, and the workgroup meets once a tile.
-// LEAD: loads are issued one tile earlier still, for D = 64, whose tiles take less time
-// than a load from beyond the L2 (16-bit: a third LDS stage; 8-bit: a second set of registers).
 template <bool KV8, bool BF16, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_pipe_kernel(const KvAttn a) {
   constexpr bool MBF = BF16 && !KV8;
   constexpr int TILE = KV_BLOCK * D * 2;
   constexpr int KS = D / 16, NV = D / 32, NK = 2 * KS, NF = 4 * NV;
   constexpr int ROWS = 128, AHEAD = D == 64 ? 2 : 1;         // slots from a fragment's read to its use
-  constexpr int LEAD = 0, STAGES = KV8 ? 2 : 2 + LEAD;
   using TK = KvTiles<KV8, D, false>;
   using TV = KvTiles<KV8, D, true>;
-  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[STAGES][TILE];
-  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[STAGES][TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[2][TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[2][TILE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
@@ -533,6 +526,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const bool live = wrow < nrows && kv_query(a, wrow) < rg.nq;      // wave-uniform
   const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
 
+  KvRows<KV8, BF16, D> qr;
+  const int rc = row < nrows ? row : nrows - 1, qi = kv_query(a, rc);
+  qr.fetch(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h);    // before the tiles
+  __builtin_amdgcn_sched_barrier(0);
   TK kt;
   TV vt;
   kt.init(a, b, hk, rg, wave, lane);
@@ -540,12 +537,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const uint32_t klds0 = lds_addr(k_lds), vlds0 = lds_addr(v_lds);
   // 8-bit: what is on its way to registers.  Block scales come by vector loads: a scalar
   // load in flight would make every wait for an LDS read wait for it, too.
-  struct Flight {
-    uint4 k[TK::UNITS], v[TV::UNITS];
-    float ks, vs;
-  };
-  Flight fa, fx;
-  Flight& fb = LEAD ? fx : fa;                               // of odd steps
+  uint4 kraw[TK::UNITS], vraw[TV::UNITS];
+  float ks = 0.f, ks_next = 0.f, vs_next = 0.f;              // ks: of this tile
   const float *ks_at = nullptr, *vs_at = nullptr;
   if constexpr (KV8) {
     long at = ((long)b * a.Hk + hk) * a.blocks + rg.t0;
@@ -553,33 +546,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     ks_at = a.ks + at, vs_at = a.vs + at;
   }
   KvUnits units;
-  float ks = 0.f;                                            // of this tile
   uint8_t mask_byte = 1;
   auto load_mask = [&](int j) __attribute__((always_inline)) {
     const int key = (rg.t0 + j) * KV_BLOCK + lane;
     mask_byte = key < rg.len ? a.mask[b * a.mask_bs + key] : 0;
   };
-  // step j: K of j + 2 + LEAD, V of j + LEAD, the key scale of j + 1 + LEAD, the mask of j + 1
-  auto feed = [&](int j, Flight& f) __attribute__((always_inline)) {
+  // step j: K of j + 2, V of j, the key scale and mask of j + 1
+  auto feed = [&](int j) __attribute__((always_inline)) {
     if constexpr (!KV8)
       if (a.mask && j + 1 < n) load_mask(j + 1);
-    if (j + 2 + LEAD < n) kt.start(klds0 + (j + 2 + LEAD) % STAGES * TILE, wave, f.k);
-    if (j + LEAD < n) {
-      vt.start(vlds0 + (j + LEAD) % STAGES * TILE, wave, f.v);
-      if constexpr (KV8) f.vs = *vs_at++;
-    }
-    if constexpr (KV8)
-      if (j + 1 + LEAD < n) f.ks = *++ks_at;
-  };
-  // K of j + 2 and V of j into LDS
-  auto settle = [&](int j, const Flight& f) __attribute__((always_inline)) {
+    if (j + 2 < n) kt.start(klds0 + (j & 1) * TILE, wave, kraw);
+    vt.start(vlds0 + (j & 1) * TILE, wave, vraw);
     if constexpr (KV8) {
-      if (j + 2 < n) TK::place(k_lds[j & 1], (_Float16)1.0f, wave, lane, f.k);
-      TV::place(v_lds[j & 1], (_Float16)units.fit(f.vs), wave, lane, f.v);
-      ks = f.ks;
-    } else if (LEAD && j + 2 + LEAD < n) {
-      static_assert(!LEAD || 2 * TK::DMA == 4, "copies of one step, which may stay in flight");
-      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      vs_next = *vs_at++;
+      if (j + 1 < n) ks_next = *++ks_at;
+    }
+  };
+  auto settle = [&](int j) __attribute__((always_inline)) {
+    if constexpr (KV8) {
+      if (j + 2 < n) TK::place(k_lds[j & 1], (_Float16)1.0f, wave, lane, kraw);
+      TV::place(v_lds[j & 1], (_Float16)units.fit(vs_next), wave, lane, vraw);
+      ks = ks_next;
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -597,11 +584,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return seen;
   };
-  // value rows of a tile whose keys are left out may hold anything
+  // stage j % 2: value rows whose keys are left out may hold anything
   auto clear = [&](int j, uint64_t seen) __attribute__((always_inline)) {
     if constexpr (!KV8) {
       if (seen != ~0ull) {
-        uint4* t = reinterpret_cast<uint4*>(v_lds[j % STAGES]);
+        uint4* t = reinterpret_cast<uint4*>(v_lds[j & 1]);
 #pragma unroll
         for (int i = 0; i < TILE / 16 / 256; ++i) {
           constexpr int ROWS_AT = 256 / (D / 8);     // rows that 256 chunks cover
@@ -617,44 +604,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int ve = 0;                                        // of O
   if (n > 0) {
     // K of tiles 0 and 1; zero in the stage that the first PV reads (its P is zero, too)
-    kt.start(klds0, wave, fa.k);
+    kt.start(klds0, wave, kraw);
     if constexpr (KV8) {
       ks = *ks_at;
-      TK::place(k_lds[0], (_Float16)1.0f, wave, lane, fa.k);
+      TK::place(k_lds[0], (_Float16)1.0f, wave, lane, kraw);
     }
     if (n > 1) {
-      kt.start(klds0 + TILE, wave, fa.k);
-      if constexpr (KV8) TK::place(k_lds[1], (_Float16)1.0f, wave, lane, fa.k);
+      kt.start(klds0 + TILE, wave, kraw);
+      if constexpr (KV8) TK::place(k_lds[1], (_Float16)1.0f, wave, lane, kraw);
     }
-    if constexpr (LEAD) feed(-1, fb);
-    else if constexpr (!KV8)
+    if constexpr (!KV8)
       if (a.mask) load_mask(0);
-    for (int i = tid; i < TILE / 16; i += 256) reinterpret_cast<uint4*>(v_lds[STAGES - 1])[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < TILE / 16; i += 256) reinterpret_cast<uint4*>(v_lds[1])[i] = make_uint4(0, 0, 0, 0);
     if constexpr (!KV8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
     uint64_t before = ~0ull;                         // what the tile before left
     if (!live) {
       // rows past the end: the wave only stages its share
       lds_barrier();
-      for (int j = 0; j < n; j += 2) {
-        clear(j - 1, before);
+      for (int j = 0; j < n; ++j) {
+        clear(j + 1, before);
         before = visible(j);
-        feed(j, fa);
-        settle(j, fb);
-        if (j + 1 < n) {
-          clear(j, before);
-          before = visible(j + 1);
-          feed(j + 1, fb);
-          settle(j + 1, fa);
-        }
+        feed(j);
+        settle(j);
       }
       clear(n - 1, before);
       return;
     }
-    KvRows<KV8, BF16, D> qr;
-    const int rc = row < nrows ? row : nrows - 1;
-    const int qi = kv_query(a, rc);
-    qr.load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h, a.scale_log2);
+    qr.finish(a.scale_log2);
     const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;                      // the last key that the row sees
     auto frag_k = [&](int stage, int f) __attribute__((always_inline)) {               // f = kb + 2 st
       if constexpr (KV8) return reinterpret_cast<const uint4*>(k_lds[stage])[((f & 1) * KS + (f >> 1)) * 64 + lane];
@@ -678,27 +655,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     };
     // sc, p: the tile's scores, the probabilities of the tile before; next, pn: the next of each
-    auto step = [&](int j, f32x16 (&sc)[2], f32x16 (&next)[2], uint4 (&p)[4], uint4 (&pn)[4], Flight& out,
-                    const Flight& in) __attribute__((always_inline)) {
+    auto step = [&](int j, f32x16 (&sc)[2], f32x16 (&next)[2], uint4 (&p)[4], uint4 (&pn)[4]) __attribute__((always_inline)) {
       const int key0 = (rg.t0 + j) * KV_BLOCK;
-      const int ks_stage = (j + 1) % STAGES, vs_stage = (j + STAGES - 1) % STAGES;
+      const int other = (j + 1) & 1;                 // stage of K of j + 1 and of V of j - 1
       constexpr int PK = NK / 8, PV = NF / 8;        // products of a slot
       uint4 kf[NK], vf[NF];
-      clear(j + STAGES - 1, before);
+      clear(j + 1, before);
       auto read = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < PK; ++e) kf[slot * PK + e] = frag_k(ks_stage, slot * PK + e);
+        for (int e = 0; e < PK; ++e) kf[slot * PK + e] = frag_k(other, slot * PK + e);
 #pragma unroll
-        for (int e = 0; e < PV; ++e) vf[slot * PV + e] = frag_v(vs_stage, slot * PV + e);
+        for (int e = 0; e < PV; ++e) vf[slot * PV + e] = frag_v(other, slot * PV + e);
       };
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) read(i);
       const uint64_t seen = visible(j);
       const float kscale = ks;
-      feed(j, out);
+      feed(j);
       rescale();
       const float c = KV8 ? kv_factor((kscale > 0.f || kscale != kscale ? kscale : 1.0f) * qr.mul) : qr.mul;
-      if (j >= edge) kv_mask<2>(sc, seen & kv_below(upto - key0 + 1), h);
+      if (j >= edge && (KV8 || seen != ~0ull)) kv_mask<2>(sc, seen & kv_below(upto - key0 + 1), h);
       kv_softmax<MBF, D, 2, true>(sc, c, s, pn, [&](int i) __attribute__((always_inline)) {
         if (i + AHEAD < 8) read(i + AHEAD);
 #pragma unroll
@@ -713,21 +689,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       });
       before = seen;
-      settle(j, in);
+      settle(j);
     };
     auto last = [&](uint4 (&p)[4]) __attribute__((always_inline)) {
       clear(n - 1, before);
       rescale();
 #pragma unroll
-      for (int f = 0; f < NF; ++f) s.o[f % NV] = kv_mfma<MBF>(frag_v((n - 1) % STAGES, f), p[f / NV], s.o[f % NV]);
+      for (int f = 0; f < NF; ++f) s.o[f % NV] = kv_mfma<MBF>(frag_v((n - 1) & 1, f), p[f / NV], s.o[f % NV]);
     };
     int j = 0;
     for (; j + 1 < n; j += 2) {
-      step(j, sa, sb, pa, pb, fa, fb);
-      step(j + 1, sb, sa, pb, pa, fb, fa);
+      step(j, sa, sb, pa, pb);
+      step(j + 1, sb, sa, pb, pa);
     }
     if (j < n) {
-      step(j, sa, sb, pa, pb, fa, fb);
+      step(j, sa, sb, pa, pb);
       last(pb);
     } else {
       last(pa);
@@ -767,6 +743,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const bool live = wrow < nrows && kv_query(a, wrow) < rg.nq;      // wave-uniform
   const int n = rg.t1 - rg.t0;                               // tiles, counted from 0 below
 
+  KvRows<KV8, BF16, D> qr[QB];
+  int upto[QB];                                      // the last key that the row sees
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = wrow + 32 * qb + l32, rc = r < nrows ? r : nrows - 1, qi = kv_query(a, rc);
+    qr[qb].fetch(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h);   // before the tiles
+    upto[qb] = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
+  }
+  __builtin_amdgcn_sched_barrier(0);
   TK kt;
   TV vt;
   kt.init(a, b, hk, rg, wave, lane);
@@ -839,15 +824,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return;
   }
-  KvRows<KV8, BF16, D> qr[QB];
   KvState<D> s[QB];
-  int upto[QB];                                      // the last key that the row sees
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const int r = wrow + 32 * qb + l32, rc = r < nrows ? r : nrows - 1;
-    const int qi = kv_query(a, rc);
-    qr[qb].load(a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs, h, a.scale_log2);
-    upto[qb] = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
+    qr[qb].finish(a.scale_log2);
     s[qb].init();
   }
   int ve = 0;                                        // of O
@@ -875,7 +855,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       s[qb].o[f & 1] = kv_mfma<MBF>(vf[f], pf[qb][f >> 1], s[qb].o[f & 1]);
     };
     auto mask = [&](int qb) __attribute__((always_inline)) {
-      if (j >= edge) kv_mask<2>(sc[qb], seen & kv_below(upto[qb] - (rg.t0 + j) * KV_BLOCK + 1), h);
+      if (j >= edge && (KV8 || seen != ~0ull)) kv_mask<2>(sc[qb], seen & kv_below(upto[qb] - (rg.t0 + j) * KV_BLOCK + 1), h);
     };
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
