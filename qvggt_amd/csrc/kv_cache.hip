@@ -56,7 +56,7 @@ template <int D, bool BF16>
 __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
     const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, uint8_t* __restrict__ k_codes,
     uint8_t* __restrict__ v_codes, float* __restrict__ k_scales, float* __restrict__ v_scales,
-    const int32_t* start_in, int32_t* lens_out, uint32_t* tickets, const int32_t* __restrict__ counts, int n, int Hk,
+    const int32_t* start_in, int32_t* lens_out, uint32_t* tickets, const int32_t* counts, int n, int Hk,
     int blocks, long k_bs, long k_ts, long k_hs, long v_bs, long v_ts, long v_hs) {
   constexpr int BYTES = KV_BLOCK * D;      // of one block's keys or values
   constexpr int HALF = 2 * D;              // threads for each of the two
@@ -188,13 +188,13 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
       for (int i = t; i < BYTES / 16; i += HALF)
         reinterpret_cast<uint4*>(codes)[i] = *reinterpret_cast<const uint4*>(stage + kv_skew(16 * i));
   }
-  // The length is written when all workgroups of the sequence have read the start, if that
-  // is the same tensor: by the last one, found by tickets that wrap to 0 by themselves (one
-  // for each head and one for the heads, on lines of their own: 376 increments of a
-  // sequence's one word took longer than the codes).
+  // The length is written when all workgroups of the sequence have read the start and the
+  // count, if one of them is the same tensor: by the last one, found by tickets that wrap to
+  // 0 by themselves (one for each head and one for the heads, on lines of their own: 376
+  // increments of a sequence's one word took longer than the codes).
   if (tid == 0) {
     bool last = head == 0 && blockIdx.x == 0;
-    if (start_in == lens_out) {
+    if (start_in == lens_out || counts == lens_out) {
       uint32_t* mine = tickets + (size_t)b * (Hk + 1) * KV_TICKET;
       last = gridDim.x == 1 || atomicInc(mine + (head + 1) * KV_TICKET, gridDim.x - 1) == gridDim.x - 1;
       if (last) last = atomicInc(mine, (uint32_t)Hk - 1) == (uint32_t)Hk - 1;

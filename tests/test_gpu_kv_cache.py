@@ -213,3 +213,42 @@ def test_append_in_a_graph_and_on_another_stream(gpu):
         both.append(k, v)
     torch.cuda.current_stream().wait_stream(st)
     both.check()
+
+
+@pytest.mark.parametrize("B,H,n", [(3, 2, 1), (2, 5, 700), (4, 1, 65)])
+def test_lens_advance_by_themselves(gpu, B, H, n):
+    """start left out, or lens itself: the length moves on once all of a sequence's workgroups have read it,
+    call after call; the same contents as with a start of its own."""
+    from qvggt_amd.kv_cache import Int8KVCache
+    g = torch.Generator(device=gpu).manual_seed(n)
+    a, b, c = (Int8KVCache(B, H, 64, 3000, device=gpu) for _ in range(3))
+    at = torch.zeros(B, dtype=torch.int32, device=gpu)
+    for i in range(4):
+        k, v = _kv(gpu, g, B, n, H, 64, torch.float16)
+        counts = torch.randint(0, n + 1, (B,), generator=g, device=gpu, dtype=torch.int32)
+        a.append(k, v, counts=counts)
+        b.append(k, v, counts=counts, start=b.lens)
+        c.append(k, v, counts=counts, start=at)
+        at = at + counts
+        assert a.lens.tolist() == b.lens.tolist() == c.lens.tolist() == at.tolist()
+    for x, y, z in zip(a.values(), b.values(), c.values()):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+@pytest.mark.parametrize("own_start", [False, True])
+def test_counts_are_lens(gpu, own_start):
+    """lens itself as the counts: written once every workgroup of the sequence has read it."""
+    from qvggt_amd.kv_cache import Int8KVCache
+    g = torch.Generator(device=gpu).manual_seed(5)
+    for _ in range(4):
+        a, b = (Int8KVCache(3, 6, 64, 4000, device=gpu) for _ in range(2))
+        for c in (a, b):
+            c.lens.copy_(torch.tensor([1900, 0, 70], dtype=torch.int32))
+        k, v = _kv(gpu, g, 3, 2000, 6, 64, torch.float16)
+        start = torch.tensor([5, 64, 0], dtype=torch.int32, device=gpu) if own_start else None
+        a.append(k, v, counts=a.lens, start=start)
+        b.append(k, v, counts=b.lens.clone(), start=start)
+        assert a.lens.tolist() == b.lens.tolist() == ([1905, 64, 70] if own_start else [3800, 0, 140])
+        n = a.lens.max().item()
+        for x, y in zip(a.values(n), b.values(n)):
+            assert torch.equal(x, y)
