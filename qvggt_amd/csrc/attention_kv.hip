@@ -1218,7 +1218,7 @@ static void kv_launch(const KvAttn& a, const KvPlan& p, hipStream_t st) {
 }
 
 // Checks and fields that both entries share.
-static int kv_common(KvAttn& a, const char* what, const void* q, void* out, int dtype, int64_t B, int64_t Lq, int64_t Lk,
+static int kv_common(KvAttn& a, const void* q, void* out, int dtype, int64_t B, int64_t Lq, int64_t Lk,
                      int64_t H, int64_t Hk, int64_t D, const int64_t* qs, const int64_t* os, float scale) {
   QV_CHECK_ARG(dtype == QV_F16 || dtype == QV_BF16, "bad dtype %d", dtype);
   QV_CHECK_ARG(D == 64 || D == 128, "head_dim must be 64 or 128 (got %lld)", (long long)D);
@@ -1281,7 +1281,7 @@ extern "C" int qv_attention_cross(const void* q, const void* k, const void* v, v
                                   const int64_t* v_strides, const int64_t* out_strides, float scale, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   qv::KvAttn a = {};
-  if (int rc = qv::kv_common(a, "attention_cross", q, out, dtype, B, Lq, Lk, H, Hk, D, q_strides, out_strides, scale))
+  if (int rc = qv::kv_common(a, q, out, dtype, B, Lq, Lk, H, Hk, D, q_strides, out_strides, scale))
     return rc;
   if (B == 0 || Lq == 0) return QV_OK;
   if (Lk > 0) {
@@ -1309,7 +1309,7 @@ extern "C" int qv_kv8_attention(const void* q, void* out, int dtype, const void*
                                 void* workspace, int64_t workspace_bytes, void* stream) {
   qv::KvAttn a = {};
   QV_CHECK_ARG(blocks > 0 && blocks <= (INT32_MAX >> 8), "bad number of blocks %lld", (long long)blocks);
-  if (int rc = qv::kv_common(a, "kv8_attention", q, out, dtype, B, Lq, blocks * qv::KV_BLOCK, H, Hk, D, q_strides,
+  if (int rc = qv::kv_common(a, q, out, dtype, B, Lq, blocks * qv::KV_BLOCK, H, Hk, D, q_strides,
                              out_strides, scale))
     return rc;
   if (B == 0 || Lq == 0) return QV_OK;

@@ -186,6 +186,37 @@ def test_cross_strides(gpu, Lq, D):
     _close(E.cross_attention(q, same, v)[1], q[1], same[1], v[1])
 
 
+@pytest.mark.parametrize("Lq", [1, 40, 200])
+def test_smaller_workspaces(gpu, monkeypatch, Lq):
+    """With less workspace than asked for the keys are split less, down to not at all."""
+    from qvggt_amd import awq_inference_engine as E
+    q, k, v = _qkv(gpu, 33, 2, Lq, 5000, 2, 1, 64, F16, 3.0)
+    full = E._kv_workspace_bytes(0, 2, Lq, 2, 1, 64, 5000)
+    want = E.cross_attention(q, k, v)
+    one = 2 * Lq * 2 * (64 * 4 + 8)
+    assert full % one == 0 and full > 3 * one
+    for size in (3 * one + 5, one, 16, 0):
+        monkeypatch.setattr(E, "_kv_workspace_bytes", lambda *shape: size)
+        out = E.cross_attention(q, k, v)
+        for b in range(2):
+            _close(out[b], q[b], k[b], v[b])
+    monkeypatch.undo()
+    assert torch.equal(E.cross_attention(q, k, v), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Lq", [1, 9, 64, 300])
+def test_cross_and_cached_agree(gpu, Lq, dtype):
+    """The cache's values as 16-bit keys and values give what the cache gives: both against
+    the oracle, causal rows as a mask."""
+    from qvggt_amd import awq_inference_engine as E
+    c = _cache(gpu, 51, 1, (700,), 2, 64, F16)
+    k, v = c.values(700, dtype=F16)
+    q = _rand(gpu, 52, 1, Lq, 4, 64)
+    _close(E.cross_attention(q, k, v)[0], q[0], k[0], v[0])
+    _check_cached(c.attention(q.to(dtype)), q.to(dtype), c)
+
+
 def test_cross_long_offsets(gpu):
     """Keys and values whose offsets pass 32 bits (a 5.2 GB buffer, 65536 elements from token to token)."""
     from qvggt_amd import awq_inference_engine as E

@@ -105,3 +105,26 @@ def test_rope_axes_non_finite_stays_in_its_pair(gpu):
     out = E.rope_axes(x, pos, E.rope_axes_plan(64, (32,), device=gpu))
     bad = ~torch.isfinite(out)
     assert bad.nonzero().tolist() == [[1, 0, 3], [1, 0, 19], [2, 1, 40]]
+
+
+@pytest.mark.parametrize("dtype,D,H,sections,layout", [(torch.float16, 64, 32, (16, 24, 24), "block"),
+                                                       (torch.bfloat16, 128, 9, (40, 48), "half"),
+                                                       (torch.float32, 64, 5, (32, 24), "block"),
+                                                       (torch.float16, 512, 3, (512,), "half")])
+def test_rope_axes_large(gpu, dtype, D, H, sections, layout):
+    """Past 64 MB whole rows are taken a lane each 8 dims: the bits of the same tokens in small
+    calls (in pieces), for a tensor of its own, inside a fused buffer and in place."""
+    from qvggt_amd import awq_inference_engine as E
+    T = (64 << 20) // (2 * H * D * torch.empty(0, dtype=dtype).element_size()) + 37
+    g = torch.Generator(device=gpu).manual_seed(D)
+    buf = torch.randn(T, H + 2, D, generator=g, device=gpu).to(dtype)
+    x = buf[:, 1:-1]
+    pos = torch.randint(-100, 100000, (T, len(sections)), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(D, sections, layout=layout, device=gpu)
+    want = torch.cat([E.rope_axes(x[i:i + 700], pos[i:i + 700], plan) for i in range(0, T, 700)])
+    _check(want[:50], x[:50], pos[:50], O.rope_pairs(sections, layout))
+    assert torch.equal(E.rope_axes(x, pos, plan), want)
+    assert torch.equal(E.rope_axes(x.contiguous(), pos, plan), want)
+    edge = buf[:, ::H + 1].clone()
+    E.rope_axes(x, pos, plan, out=x)
+    assert torch.equal(x, want) and torch.equal(buf[:, ::H + 1], edge)

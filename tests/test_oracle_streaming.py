@@ -160,3 +160,58 @@ def test_attention_kv_refusals():
                           ((q,), {}, "GPU only")):
         with pytest.raises(RuntimeError, match=msg):
             c.attention(*args, **kw)
+
+
+def test_c_entries_refuse():
+    """Bad arguments end at the C entries with a message, before any device work (pointers here are never followed)."""
+    import ctypes as C
+
+    from qvggt_amd import _lib
+    lib = _lib.load()
+    st = (C.c_int64 * 3)(64 * 8, 64, 64)
+    odd = (C.c_int64 * 3)(64 * 8, 60, 64)
+    p = 1 << 20
+
+    def refused(rc, what):
+        assert rc == -1 and what in lib.qv_last_error().decode(), (rc, lib.qv_last_error())
+
+    rope = lambda **kw: lib.qv_rope_axes(*{**dict(x=p, out=p, dt=0, pos=p, turns=p, sec=(C.c_int64 * 2)(32, 32), axes=2, layout=0,
+                                                  T=5, H=2, D=64, a=128, b=64, c=128, d=64, s=None), **kw}.values())
+    for kw, what in ((dict(dt=7), "dtype"), (dict(axes=0), "axes"), (dict(axes=5), "axes"), (dict(layout=2), "layout"),
+                     (dict(D=63), "shape"), (dict(H=5000), "shape"), (dict(sec=(C.c_int64 * 2)(31, 2)), "section"),
+                     (dict(sec=(C.c_int64 * 2)(64, 2)), "sections"), (dict(x=None), "null"), (dict(turns=None), "null"),
+                     (dict(x=p + 1), "aligned")):
+        refused(rope(**kw), what)
+    assert rope(T=0) == 0
+    app = lambda **kw: lib.qv_kv8_append(*{**dict(k=p, v=p, dt=0, kc=p, vc=p, ks=p, vs=p, start=p, lens=p, tick=p, counts=None, B=1,
+                                                  n=5, Hk=2, D=64, blocks=3, kst=st, vst=st, s=None), **kw}.values())
+    for kw, what in ((dict(D=32), "head_dim"), (dict(n=193), "do not fit"), (dict(dt=2), "dtype"), (dict(kst=odd), "strides"),
+                     (dict(k=p + 2), "aligned"), (dict(kc=p + 8), "aligned"), (dict(lens=None), "null"), (dict(blocks=0), "cache shape"),
+                     (dict(B=40000), "cache shape"), (dict(blocks=1 << 24), "cache shape"), (dict(k=None), "null")):
+        refused(app(**kw), what)
+    assert app(B=0) == 0
+    val = lambda **kw: lib.qv_kv8_values(*{**dict(kc=p, vc=p, ks=p, vs=p, lens=p, first=None, ko=p, vo=p, dt=2, B=1, n=5, Hk=2, D=64,
+                                                  blocks=3, s=None), **kw}.values())
+    for kw, what in ((dict(dt=3), "dtype"), (dict(n=-1), "number of tokens"), (dict(ko=None), "null"), (dict(vo=p + 4), "aligned")):
+        refused(val(**kw), what)
+    assert val(n=0) == 0
+    cross = lambda **kw: lib.qv_attention_cross(*{**dict(q=p, k=p, v=p, out=p, dt=0, lens=None, mask=None, ms=0, B=1, Lq=5, Lk=9, H=4,
+                                                         Hk=2, D=64, qs=st, ks=st, vs=st, os=st, scale=0.1, ws=None, wb=0, s=None),
+                                                  **kw}.values())
+    far = (C.c_int64 * 3)(64, 1 << 25, 64)
+    for kw, what in ((dict(dt=2), "dtype"), (dict(D=96), "head_dim"), (dict(Hk=3), "shape"), (dict(scale=0.0), "scale"),
+                     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(q=p + 8), "aligned"),
+                     (dict(k=p + 8), "aligned"), (dict(qs=odd), "strides"), (dict(ks=odd), "strides"), (dict(vs=far), "token strides"),
+                     (dict(ks=(C.c_int64 * 3)(64, 0, 64)), "token strides"), (dict(v=None), "null"), (dict(out=None), "null"),
+                     (dict(B=70000), "grid"), (dict(Lq=1 << 27, H=256, Hk=2), "rows")):
+        refused(cross(**kw), what)
+    assert cross(B=0) == 0 and cross(Lq=0) == 0
+    att = lambda **kw: lib.qv_kv8_attention(*{**dict(q=p, out=p, dt=0, kc=p, vc=p, ks=p, vs=p, lens=p, counts=None, causal=0, B=1,
+                                                     Lq=5, H=4, Hk=2, D=64, blocks=3, keys=100, qs=st, os=st, scale=0.1, ws=None,
+                                                     wb=0, s=None), **kw}.values())
+    for kw, what in ((dict(blocks=0), "blocks"), (dict(lens=None), "null"), (dict(kc=p + 8), "aligned"), (dict(D=32), "head_dim"),
+                     (dict(scale=-1.0), "scale"), (dict(H=5), "shape")):
+        refused(att(**kw), what)
+    need = lib.qv_attention_kv_workspace
+    assert need(1, 1, 1, 8, 1, 96, 5000) == 0 and need(1, 1, 1, 8, 3, 64, 5000) == 0 and need(1, 0, 1, 8, 1, 64, 5000) == 0
+    assert need(1, 1, 1, 8, 1, 64, 64) == 0 and need(0, 1, 1, 8, 1, 64, 100000) > 0
