@@ -11,13 +11,15 @@
 // scores, which are the second product's operand without a shuffle.  One running
 // reference m and sum l per row; m moves only when a score passes it by far.
 //
-// Forms:
-//  * wide: 4 waves, each 32 or 64 rows of its own, K / V tiles of the workgroup in LDS
-//    (16-bit: LDS DMA; 8-bit: codes through registers, converted once by the whole
+// Forms, by the rows of a key head:
+//  * wide: over 128 rows of D = 64; 4 waves of 64 rows, K / V tiles of the workgroup in
+//    LDS (16-bit: LDS DMA; 8-bit: codes through registers, converted once by the whole
 //    workgroup, stored in fragment order);
+//  * pipelined: D = 128, or 33 to 128 rows of D = 64; 4 waves of 32 rows on the same
+//    tiles, the next tile's scores and the last one's products beside a softmax;
 //  * step: up to 32 rows, every wave its own tiles of the key range (16-bit: LDS
 //    areas of its own; 8-bit: fragments straight from memory), joined in LDS.
-// In both the key range may be split over workgroups, joined by a second kernel.
+// In all of them the key range may be split over workgroups, joined by a second kernel.
 //
 // 8-bit values: scores are products of 16-bit queries with whole numbers, the key
 // block's scale goes into c.  bf16 queries become fp16 under a power of two of their
@@ -501,6 +503,13 @@ struct KvTiles {
 // 4 waves of 32 rows.  Beside tile j's softmax run the QK of tile j + 1 and the PV of tile
 // j - 1, a few of each in every slot, so that no product stands alone.  K is in LDS two
 // tiles ahead, V comes with its own tile, and the workgroup meets once a tile.
+// Bound by issue: a wave's tile of D = 128 is 32 MFMAs and 32 exponentials with their
+// multiply-adds, conversions and sums, and an MFMA takes 10 to 18 cycles of vector issue too.  Two workgroups a CU need
+// 2.1 us a tile, one alone 1.24: with the chip full 1050 TF/s over 16-bit and 950 over 8-bit
+// keys (a large fp16 matrix product of the library: 1170).  64 rows a wave would halve
+// the LDS reads, but at D = 128 O and the queries leave no registers for it: with O in
+// accumulation registers 1374 queries of 16 heads took 112 us instead of 87.  For 33 to
+// 128 rows of D = 64 half of a wide workgroup's rows would be empty.
 template <bool KV8, bool BF16, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_pipe_kernel(const KvAttn a) {
   constexpr bool MBF = BF16 && !KV8;
@@ -718,6 +727,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // 4 waves of 64 rows (two blocks of 32), D = 64: every fragment that is read from LDS and
 // every code that is decoded serves twice the rows.  Inside a tile the second block's QK
 // runs beside the first one's softmax, the first one's PV beside the second's.
+// Bound by issue: 64 x 64 scores a tile and wave cost 32 MFMAs and 64 exponentials of 8
+// cycles with their multiply-adds, conversions and sums.  Two workgroups a CU need 2.43 us a
+// tile, one alone 1.48: 890 TF/s over 16-bit keys and 850 over the cache with the chip full.
+// 1374 queries of 16 heads over 10992 keys: 91 us and 7 of join under a trace (90 in all
+// without); over a cache of 43968 tokens 349 and 7 (323 in all without).
 template <bool KV8, bool BF16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_wide_kernel(const KvAttn a) {
   constexpr int D = 64, QB = 2;
@@ -890,6 +904,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // ------------------------------------------------------------------ step form
+// Bound by the bytes of the keys and values: 16 sequences of 8000 cached tokens, 8 heads of
+// 128 dims, read at 6.2 TB/s (a large copy moves 5.2, a read alone more).  16-bit D = 64 takes 8
+// waves: 8 x 16 heads over 1374 keys 11.3 us, 4.0 TB/s.  A wave has tiles of its own,
+// so that none waits for another before the end; 32 rows fill the MFMA's columns however few
+// there are, and cost nothing that the bytes would not.
 constexpr int kv_step_waves(bool kv8, int d) { return !kv8 && d == 64 ? 8 : 4; }
 template <bool KV8, bool BF16, int D>
 struct KvStep {
@@ -900,7 +919,9 @@ struct KvStep {
   static constexpr int LDS = KV8 ? WAVES * 32 * D * 4 : WAVES * 4 * TILE;   // the join's rows / 2 stages of K and V
 };
 template <bool KV8, bool BF16, int D>
-__global__ __launch_bounds__(64 * kv_step_waves(KV8, D)) __attribute__((amdgpu_waves_per_eu(KV8 || D == 64 ? 2 : 1, KV8 || D == 64 ? 2 : 1))) void kv_attn_step_kernel(const KvAttn a) {
+__global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
+    __attribute__((amdgpu_waves_per_eu(KV8 || D == 64 ? 2 : 1, KV8 || D == 64 ? 2 : 1))) void
+    kv_attn_step_kernel(const KvAttn a) {
   using C = KvStep<KV8, BF16, D>;
   constexpr bool MBF = BF16 && !KV8;
   constexpr int KS = D / 16, NV = D / 32, KB = C::KB, KT = C::KT, TILE = C::TILE;
@@ -1118,7 +1139,8 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D)) __attribute__((amdgpu_w
 
 // ------------------------------------------------------------------ join of the splits
 // A thread takes 4 dims of one row: sum of the splits' quotients, weighted by l 2^m, with
-// a running maximum, so that all loads are on their way at once.
+// a running maximum, so that all loads are on their way at once.  Some 4 us for few rows (the
+// launch and two dependent reads), 7 us for 5 splits of 1374 queries of 16 heads of 64 dims.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttn a) {
   const int b = blockIdx.z, hk = blockIdx.y;
