@@ -196,9 +196,11 @@ __global__ __launch_bounds__(4 * D) void kv8_append_kernel(
   // count, if one of them is the same tensor: by the last one, found by tickets that wrap to
   // 0 by themselves (one for each head and one for the heads, on lines of their own: 376
   // increments of a sequence's one word took longer than the codes).
+  const bool turn = start_in == lens_out || counts == lens_out;
+  if (turn) __syncthreads();               // a workgroup without tokens has met no barrier so far
   if (tid == 0) {
     bool last = head == 0 && blockIdx.x == 0;
-    if (start_in == lens_out || counts == lens_out) {
+    if (turn) {
       uint32_t* mine = tickets + (size_t)b * (Hk + 1) * KV_TICKET;
       last = gridDim.x == 1 || atomicInc(mine + (head + 1) * KV_TICKET, gridDim.x - 1) == gridDim.x - 1;
       if (last) last = atomicInc(mine, (uint32_t)Hk - 1) == (uint32_t)Hk - 1;

@@ -123,7 +123,8 @@ class Int8KVCache:
         causal: the queries are the sequence's last n tokens, each sees the tokens
         up to its own.  counts int32 (B,): how many of the n queries each sequence
         has; the rows of ``out`` behind them are left as they were (zero in a new
-        out).  A query that sees no token gives zeros.  Returns (B, n, heads, head_dim)."""
+        out).  A query that sees no token gives zeros.  ``out`` must not overlap q.
+        Returns (B, n, heads, head_dim)."""
         what = "Int8KVCache.attention"
         dt, scale = _kv_query(q, self.kv_heads, out, scale, what)
         B, n, H, D = q.shape

@@ -252,3 +252,21 @@ def test_counts_are_lens(gpu, own_start):
         n = a.lens.max().item()
         for x, y in zip(a.values(n), b.values(n)):
             assert torch.equal(x, y)
+
+
+def test_many_workgroups_without_tokens(gpu):
+    """Sequences of a few tokens, some of none, in a launch for thousands, lens as the start: workgroups
+    that find nothing to do read the start too before it moves."""
+    from qvggt_amd.kv_cache import Int8KVCache
+    g = torch.Generator(device=gpu).manual_seed(8)
+    a, b = (Int8KVCache(7, 9, 64, 6400, device=gpu) for _ in range(2))
+    at = torch.zeros(7, dtype=torch.int32, device=gpu)
+    for i in range(6):
+        k, v = _kv(gpu, g, 7, 5000, 9, 64, torch.float16)
+        counts = torch.tensor([0, 1, 63, 64, 65, 130, 2 * i], dtype=torch.int32, device=gpu)
+        a.append(k, v, counts=counts)
+        b.append(k, v, counts=counts, start=at)
+        at = at + counts
+        assert a.lens.tolist() == b.lens.tolist() == at.tolist()
+    for x, y in zip(a.values(800), b.values(800)):
+        assert torch.equal(x, y)
