@@ -134,12 +134,20 @@ struct KvUnits {
         if (e > top) top = e;
       }
     }
-    return __builtin_ldexpf(s, -ve);    // NaN stays NaN
+    return s > 0.f ? __builtin_ldexpf(s, -ve) : 0.f;
   }
 };
 
-// Key-scale factor of the scores; kept off 0 so that a masked score (-inf) times it stays -inf.
-__device__ __forceinline__ float kv_factor(float c) { return c < 1e-37f ? 1e-37f : c; }
+// What the scores of a block with key scale ks are multiplied by; kept off 0 so that a masked
+// score (-inf) times it stays -inf.
+__device__ __forceinline__ float kv_factor(float ks, float mul) {
+  const float c = (ks > 0.f ? ks : 1.0f) * mul;
+  return c < 1e-37f ? 1e-37f : c;
+}
+
+// A block marked by a NaN scale goes into the products as numbers, for a NaN there would
+// reach rows that do not see the block (0 * NaN); the sums of those that do become NaN.
+__device__ __forceinline__ bool kv_marked(float ks, float vs) { return ks != ks || vs != vs; }
 
 // The fragments of one wave's 32 rows, and what their scores are multiplied by.
 template <bool KV8, bool BF16, int D>
@@ -504,10 +512,10 @@ struct KvTiles {
 // j - 1, a few of each in every slot, so that no product stands alone.  K is in LDS two
 // tiles ahead, V comes with its own tile, and the workgroup meets once a tile.
 // Bound by issue: a wave's tile of D = 128 is 32 MFMAs and 32 exponentials with their
-// multiply-adds, conversions and sums, and an MFMA takes 10 to 18 cycles of vector issue too.  Two workgroups a CU need
-// 2.1 us a tile, one alone 1.24: with the chip full 1050 TF/s over 16-bit and 950 over 8-bit
-// keys (a large fp16 matrix product of the library: 1170).  64 rows a wave would halve
-// the LDS reads, but at D = 128 O and the queries leave no registers for it: with O in
+// multiply-adds, conversions and sums, and an MFMA takes 10 to 18 cycles of vector
+// issue too.  Two workgroups a CU need 2.1 us a tile, one alone 1.24: with the chip full
+// 1050 TF/s over 16-bit and 950 over 8-bit keys (a large fp16 matrix product of the
+// library: 1170).  64 rows a wave would halve the LDS reads, but at D = 128 O and the queries leave no registers for it: with O in
 // accumulation registers 1374 queries of 16 heads took 112 us instead of 87.  For 33 to
 // 128 rows of D = 64 half of a wide workgroup's rows would be empty.
 template <bool KV8, bool BF16, int D>
@@ -682,7 +690,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const float kscale = ks;
       feed(j);
       rescale();
-      const float c = KV8 ? kv_factor((kscale > 0.f || kscale != kscale ? kscale : 1.0f) * qr.mul) : qr.mul;
+      const float c = KV8 ? kv_factor(kscale, qr.mul) : qr.mul;
       if (j >= edge && (KV8 || seen != ~0ull)) kv_mask<2>(sc, seen & kv_below(upto - key0 + 1), h);
       kv_softmax<MBF, D, 2, true>(sc, c, s, pn, [&](int i) __attribute__((always_inline)) {
         if (i + AHEAD < 8) read(i + AHEAD);
@@ -699,6 +707,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       });
       before = seen;
       settle(j);
+      if constexpr (KV8)
+        if (kv_marked(kscale, vs_next) && (seen & kv_below(upto - key0 + 1))) s.l = __builtin_nanf("");
     };
     auto last = [&](uint4 (&p)[4]) __attribute__((always_inline)) {
       clear(n - 1, before);
@@ -780,6 +790,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   KvUnits units;
   float ks = 0.f, ks_next = 0.f, vs_next = 0.f;
+  bool marked = false;
   uint8_t mask_byte = 1;
   // the tile on its way (into stage j % 2), and into place
   auto feed = [&](int j) __attribute__((always_inline)) {
@@ -796,7 +807,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (KV8) {
       TK::place(k_lds[j & 1], (_Float16)1.0f, wave, lane, kraw);
       TV::place(v_lds[j & 1], (_Float16)units.fit(vs_next), wave, lane, vraw);
-      ks = ks_next;
+      ks = ks_next, marked = kv_marked(ks_next, vs_next);
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -851,8 +862,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const uint64_t seen = visible(j);
     float c[QB];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) c[qb] = KV8 ? kv_factor((ks > 0.f || ks != ks ? ks : 1.0f) * qr[qb].mul) : qr[qb].mul;
+    for (int qb = 0; qb < QB; ++qb) c[qb] = KV8 ? kv_factor(ks, qr[qb].mul) : qr[qb].mul;
     if constexpr (KV8) {
+      if (marked) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+          if (seen & kv_below(upto[qb] - (rg.t0 + j) * KV_BLOCK + 1)) s[qb].l = __builtin_nanf("");
+      }
       if (units.ve != ve) {
         const float by = __builtin_ldexpf(1.0f, ve - units.ve);
 #pragma unroll
@@ -993,7 +1009,8 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
           sc[kb] = kv_mfma<MBF>(lo, qr.f[2 * u], u == 0 ? f32x16{} : sc[kb]);
           sc[kb] = kv_mfma<MBF>(hi, qr.f[2 * u + 1], sc[kb]);
         }
-      const float c = kv_factor((ks > 0.f || ks != ks ? ks : 1.0f) * qr.mul);
+      const float c = kv_factor(ks, qr.mul);
+      if (kv_marked(ks, vs) && (seen & kv_below(upto - key0 + 1))) s.l = __builtin_nanf("");
       const _Float16 f = (_Float16)units.fit(vs);
       __builtin_amdgcn_sched_barrier(0);
       if (more) {

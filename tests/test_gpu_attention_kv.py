@@ -404,6 +404,28 @@ def test_cached_marked_block(gpu):
             assert torch.equal(bad, want)
 
 
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Lq,past", [(1, 191), (3, 190), (80, 190), (300, 190), (80, 4000), (300, 9000)])
+def test_cached_marked_block_behind_causal_queries(gpu, Lq, past, D, which):
+    """A NaN of the last token marks its block: queries that see a token of the block come
+    back NaN, the ones before it as if it were not there, tiles they share included."""
+    c = _cache(gpu, 61, 1, (past,), 2, D, F16, capacity=past + Lq)
+    kv = [_rand(gpu, 62 + i, 1, Lq, 2, D) for i in range(2)]
+    kv[which][0, -1, 1, 3] = float("nan")
+    c.append(*kv)
+    q = _rand(gpu, 64, 1, Lq, 4, D)
+    out = c.attention(q, causal=True)
+    last = past + Lq - 1
+    sees = past + torch.arange(Lq, device=gpu) >= last // 64 * 64
+    want = torch.zeros(1, Lq, 4, D, dtype=torch.bool, device=gpu)
+    want[:, sees, 2:] = True
+    assert torch.equal(torch.isnan(out), want) and torch.isfinite(out[~want]).all()
+    clean = (~sees).nonzero()[:, 0].cpu().numpy()
+    if len(clean):
+        _check_cached(out, q, c, causal=True, rows=clean)
+
+
 def test_cached_scale_argument_and_strides(gpu):
     c = _cache(gpu, 21, 2, (150, 90), 2, 128, F16)
     for Lq in (1, 60):
