@@ -119,7 +119,9 @@ __device__ __forceinline__ void kv_decode(const uint4& u, f16x2 f, uint4& lo, ui
 }
 
 // The scale's part of 2^ve, moving ve where the block needs it (the same in all
-// lanes).  top: the largest ve so far.
+// lanes).  top: the largest ve so far.  O moves with it in 32 bits: a row keeps what is
+// above some 2^-100 of the largest scale among its tile's blocks, its own or not (fp16
+// inputs span 2^40; bf16 ones could pass it).
 struct KvUnits {
   int ve = 0, top = -1000;
   bool any = false;

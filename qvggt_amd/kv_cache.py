@@ -23,10 +23,10 @@ class Int8KVCache:
 
     Each block of 64 tokens has one scale for each head: the smallest number
     of four significant bits that is at least amax / 127 (so that a cached value,
-    code * scale, is an fp16 number and is used without a further rounding).  A
-    block that is filled by several calls keeps the largest scale that it
-    needed, and its earlier codes are rounded again when that grows.  A NaN or
-    infinity makes all of its (block, head) NaN until the block is begun again.
+    code * scale, has the 11 bits of an fp16 number, and attention uses it without a
+    further rounding).  A NaN or infinity makes all of its (block, head) NaN, and what
+    attends to a token of it, until the block is begun again.  A block that is filled by several calls keeps the largest scale that it
+    needed, and its earlier codes are rounded again when that grows.
 
     ``lens`` (int32, on the GPU) holds the tokens of each sequence.  Calls only
     enqueue work, in stream order, and can be captured into graphs: a replayed
@@ -96,7 +96,8 @@ class Int8KVCache:
     def values(self, n: int | None = None, first: torch.Tensor | None = None, dtype: torch.dtype = torch.float32):
         """The cached (keys, values) of n tokens (default: the capacity) of each sequence
         from token first[b] (int32 (B,); default 0) on, (B, n, kv_heads, head_dim);
-        zero behind ``lens``.  float32 and, for fp16 inputs, float16 hold them exactly."""
+        zero behind ``lens``.  float32 holds them exactly, float16 those of blocks whose
+        largest lies between 2^-14 and 2^15 (a value may come back half a step larger)."""
         what = "Int8KVCache.values"
         n = self.capacity if n is None else n
         if not 0 <= n <= 64 << 23:
