@@ -252,6 +252,105 @@ __global__ __launch_bounds__(256) void rope_axes_rows_kernel(
   }
 }
 
+// The same for 16-bit types and sections that leave pieces of 1 or 2 dims: rows are read and
+// written whole as above, and turned in LDS in between, a pair to a lane, the pairs of a row
+// next to each other (no bank meets twice).  Each wave works on rows of its own, and all
+// its loads of a round come before its stores: x and out may be the same.  43968 tokens
+// of 32 heads of 64 fp16 dims, 10 + 26 + 28 by axis: 72 us, 5.0 TB/s.
+template <int DT>
+__global__ __launch_bounds__(256) void rope_axes_staged_kernel(
+    const uint8_t* x, uint8_t* out, const int32_t* __restrict__ pos, int axes, const double* __restrict__ turns, RopeAxes ra,
+    long T, int H, int pairs, int TB, uint32_t h_mul, long x_ts, long x_hs, long o_ts, long o_hs) {
+  typedef RopePiece<DT, 8> Piece;
+  constexpr int ES = Piece::ES, K = 4;               // pairs of a lane in each 512 dims of a wave
+  __shared__ float2 table[ROPE_TABLE];
+  __shared__ __attribute__((aligned(16))) uint8_t stage[4 * ROPE_UNITS * 512 * ES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long tok0 = (long)blockIdx.x * TB;
+  const int ntok = (int)(T - tok0 < TB ? T - tok0 : TB);
+  const int lanes = pairs / 4, per_wave = 64 / lanes;                // of a row; rows of 512 dims
+  const int rows = ntok * H, step = 4 * per_wave;
+  const int mine = wave * per_wave, dim0 = lane % lanes * 8;
+  uint8_t* own_stage = stage + wave * (ROPE_UNITS * 512 * ES);
+  x += tok0 * x_ts * ES;
+  out += tok0 * o_ts * ES;
+  Piece own[ROPE_UNITS];
+  auto fetch = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int row = base + step * i + mine + lane / lanes;
+      if (row < rows) {
+        const int tok = h_mul ? (int)__umulhi((uint32_t)row, h_mul) : row;
+        own[i].load(x + (tok * x_ts + (row - tok * H) * x_hs + dim0) * ES);
+      }
+    }
+  };
+  fetch(0);
+  // pair k of the lane: row and pair in the 512 dims, its dims (-1: copied)
+  int at[K], pair[K], lo[K], hi[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int q = 64 * k + lane;
+    at[k] = q / pairs, pair[k] = q % pairs;
+    int dim = ra.lo0[0] + pair[k], g = ra.gap[0], ax = ra.axis[0];
+#pragma unroll
+    for (int c = 1; c < 5; ++c)
+      if (c < ra.chunks && pair[k] >= ra.pair0[c]) dim = ra.lo0[c] + pair[k] - ra.pair0[c], g = ra.gap[c], ax = ra.axis[c];
+    lo[k] = ax < 0 ? -1 : (at[k] * 2 * pairs + dim) * ES;
+    hi[k] = lo[k] + g * ES;
+  }
+  for (int e = tid; e < ntok * pairs; e += 256) {
+    const int tok = e / pairs, p = e - tok * pairs;
+    int ax = ra.axis[0];
+#pragma unroll
+    for (int c = 1; c < 5; ++c)
+      if (c < ra.chunks && p >= ra.pair0[c]) ax = ra.axis[c];
+    float s = 0.f, c = 1.f;
+    if (ax >= 0) {
+      const double t = (double)pos[(tok0 + tok) * axes + ax] * turns[p];
+      sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    }
+    table[e] = make_float2(c, s);
+  }
+  __syncthreads();
+  for (int base = 0; base < rows; base += step * ROPE_UNITS) {
+    if (base) fetch(base);
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) own[i].store(own_stage + (i * 512 + lane * 8) * ES);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's other lanes read it
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      uint8_t* dims = own_stage + i * 512 * ES;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int row = base + step * i + mine + at[k];
+        if (row < rows && lo[k] >= 0) {
+          const int tok = h_mul ? (int)__umulhi((uint32_t)row, h_mul) : row;
+          const float2 cs = table[tok * pairs + pair[k]];
+          RopePiece<DT, 1> a, b;
+          a.load(dims + lo[k]);
+          b.load(dims + hi[k]);
+          const float l = a.get(0), h = b.get(0);
+          a.set(0, __builtin_fmaf(l, cs.x, -(h * cs.y)));
+          b.set(0, __builtin_fmaf(h, cs.x, l * cs.y));
+          a.store(dims + lo[k]);
+          b.store(dims + hi[k]);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < ROPE_UNITS; ++i) {
+      const int row = base + step * i + mine + lane / lanes;
+      if (row < rows) {
+        const int tok = h_mul ? (int)__umulhi((uint32_t)row, h_mul) : row;
+        own[i].load(own_stage + (i * 512 + lane * 8) * ES);
+        own[i].store(out + (tok * o_ts + (row - tok * H) * o_hs + dim0) * ES);
+      }
+    }
+  }
+}
+
 template <int DT>
 static void rope_axes_launch(int vec, unsigned grid, hipStream_t st, const void* x, void* out, const int32_t* pos, int axes,
                              const double* turns, const RopeAxes& ra, long T, int H, int pairs, int TB,
@@ -262,6 +361,11 @@ static void rope_axes_launch(int vec, unsigned grid, hipStream_t st, const void*
   if (vec == 0)
     hipLaunchKernelGGL((rope_axes_rows_kernel<DT>), dim3(grid), dim3(256), 0, st, (const uint8_t*)x, (uint8_t*)out, pos, axes,
                        turns, ra, T, H, pairs, TB, mul, x_ts, x_hs, o_ts, o_hs);
+  else if (vec == 16) {
+    if constexpr (DT != QV_F32)
+      hipLaunchKernelGGL((rope_axes_staged_kernel<DT>), dim3(grid), dim3(256), 0, st, (const uint8_t*)x, (uint8_t*)out, pos,
+                         axes, turns, ra, T, H, pairs, TB, mul, x_ts, x_hs, o_ts, o_hs);
+  }
   else if (vec == 8) QV_ROPE(8);
   else if (vec == 4) QV_ROPE(4);
   else if (vec == 2) QV_ROPE(2);
@@ -322,14 +426,17 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   }
   QV_CHECK_ARG((uintptr_t)x % es == 0 && (uintptr_t)out % es == 0, "x and out must be aligned to their type");
   const int pairs = (int)(D / 2);
-  // whole rows: 8 dims a lane, rows within a wave, chunks in fours, and enough of them that
-  // bytes count (T x 32 heads of 64 fp16 dims: 43968 tokens 65 us, in pieces 70; 1374
-  // tokens 6.4 and 5.5)
+  // whole rows: 8 dims a lane, rows within a wave, and enough of them that bytes count.  T x 32
+  // heads of 64 fp16 dims: with chunks in fours 65 us at 43968 tokens, in pieces 70, but 6.4 and
+  // 5.5 at 1374; with pieces of 1 or 2 dims staged in LDS 72, in pieces 132 and 94 (10992 tokens:
+  // 20, in pieces 27 and 21; 344 tokens: 6.0, in pieces 5.1 and 4.3).  32-bit types gain nothing
+  // by the stage (146, in pieces of 1 152, of 2 142 against 138).
   const int wide = 8 * es < 16 ? 8 * es : 16;
-  const bool rows = 2 * T * H * D * es > (64 << 20) && vec >= 4 && D >= 64 && D <= 512 && (D & (D - 1)) == 0 && x_token_stride % 8 == 0 &&
-                    x_head_stride % 8 == 0 && out_token_stride % 8 == 0 && out_head_stride % 8 == 0 &&
-                    (uintptr_t)x % wide == 0 && (uintptr_t)out % wide == 0;
-  const int64_t per_tok = rows ? H * (D / 8) : H * (pairs / vec);
+  const bool whole = 2 * T * H * D * es > (64 << 20) && D >= 64 && D <= 512 && (D & (D - 1)) == 0 &&
+                     x_token_stride % 8 == 0 && x_head_stride % 8 == 0 && out_token_stride % 8 == 0 &&
+                     out_head_stride % 8 == 0 && (uintptr_t)x % wide == 0 && (uintptr_t)out % wide == 0;
+  const bool rows = whole && vec >= 4, staged = whole && vec < 4 && es == 2;
+  const int64_t per_tok = rows || staged ? H * (D / 8) : H * (pairs / vec);
   // tokens of a workgroup: one round of pieces (1024), at most the table, and
   // enough workgroups to fill the chip
   int64_t tb = 256 * qv::ROPE_UNITS / per_tok;
@@ -338,8 +445,9 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   if (tb < 1) tb = 1;
   const int64_t grid = (T + tb - 1) / tb;
   const auto mul = [](int64_t n) { return n == 1 ? 0u : (uint32_t)((1ull << 32) / n + 1); };
-  const uint32_t per_tok_mul = tb == 1 ? 0u : mul(per_tok), second = rows ? mul(H) : mul(pairs / vec);
+  const uint32_t per_tok_mul = tb == 1 ? 0u : mul(per_tok), second = rows || staged ? mul(H) : mul(pairs / vec);
   if (rows) vec = 0;
+  if (staged) vec = 16;
   QV_CHECK_ARG(grid <= INT32_MAX && per_tok * tb <= INT32_MAX / 2, "too many tokens or heads");
 #define QV_ARGS                                                                                                       \
   vec, (unsigned)grid, (hipStream_t)stream, x, out, positions, (int)axes, turns, ra, (long)T, (int)H, pairs, (int)tb, \

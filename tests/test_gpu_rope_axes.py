@@ -110,9 +110,16 @@ def test_rope_axes_non_finite_stays_in_its_pair(gpu):
 @pytest.mark.parametrize("dtype,D,H,sections,layout", [(torch.float16, 64, 32, (16, 24, 24), "block"),
                                                        (torch.bfloat16, 128, 9, (40, 48), "half"),
                                                        (torch.float32, 64, 5, (32, 24), "block"),
-                                                       (torch.float16, 512, 3, (512,), "half")])
+                                                       (torch.float16, 512, 3, (512,), "half"),
+                                                       (torch.float16, 64, 32, (10, 26, 28), "half"),
+                                                       (torch.bfloat16, 64, 31, (12, 20, 20), "block"),
+                                                       (torch.bfloat16, 128, 9, (22, 50, 56), "half"),
+                                                       (torch.float16, 512, 3, (510,), "block"),
+                                                       (torch.float16, 128, 1, (30, 34), "block"),
+                                                       (torch.float32, 64, 5, (10, 26, 28), "half"),
+                                                       (torch.float16, 256, 2, (6, 250), "half")])
 def test_rope_axes_large(gpu, dtype, D, H, sections, layout):
-    """Past 64 MB whole rows are taken a lane each 8 dims: the bits of the same tokens in small
+    """Past 64 MB whole rows are taken, a lane each 8 dims, turned in registers or in LDS: the bits of the same tokens in small
     calls (in pieces), for a tensor of its own, inside a fused buffer and in place."""
     from qvggt_amd import awq_inference_engine as E
     T = (64 << 20) // (2 * H * D * torch.empty(0, dtype=dtype).element_size()) + 37
