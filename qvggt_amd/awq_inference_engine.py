@@ -792,8 +792,8 @@ def rope_axes_plan(head_dim: int, sections, base: float = 100.0, layout: str = "
 
 
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, plan: RopeAxesPlan, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Rotary positions of several axes on x (T, H, D), fp16 / bf16 / fp32, any
-    token and head strides (e.g. the q and k heads of a fused qkv buffer,
+    """Rotary positions of several axes on x (T, H, D), fp16 / bf16 / fp32, up to
+    4096 heads of up to 1024 dims, any token and head strides (e.g. the q and k heads of a fused qkv buffer,
     ``qkv.view(T, 3 * H, D)[:, :2 * H]``).
 
     positions int32 (T, axes).  ``out=x`` rotates in place; otherwise out must not

@@ -25,8 +25,9 @@ class Int8KVCache:
     of four significant bits that is at least amax / 127 (so that a cached value,
     code * scale, has the 11 bits of an fp16 number, and attention uses it without a
     further rounding).  A NaN or infinity makes all of its (block, head) NaN, and what
-    attends to a token of it, until the block is begun again.  A block that is filled by several calls keeps the largest scale that it
-    needed, and its earlier codes are rounded again when that grows.
+    attends to a token of it, until the block is begun again.  A block that is
+    filled by several calls keeps the largest scale that it needed, and its
+    earlier codes are rounded again when that grows.
 
     ``lens`` (int32, on the GPU) holds the tokens of each sequence.  Calls only
     enqueue work, in stream order, and can be captured into graphs: a replayed
