@@ -84,8 +84,9 @@ struct RopePiece {
 
 // token tile TB: TB * pairs table entries (at most ROPE_TABLE) and TB * H * groups
 // pieces of x, taken ROPE_UNITS a thread at a time.  per_tok_mul, groups_mul:
-// floor(2^32 / n) + 1 for the pieces of a token and of a head (0: one token, one piece),
-// which divide exactly while the dividend times n is below 2^32.
+// floor(2^32 / n) + 1 for the pieces of a token and of a head (0 for n = 1: the
+// dividend itself), which divide exactly while the dividend times n is below 2^32;
+// a workgroup of one token, whose pieces may pass that, does not divide by them.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void rope_axes_kernel(
     const uint8_t* x, uint8_t* out, const int32_t* __restrict__ pos, int axes, const double* __restrict__ turns, RopeAxes ra,
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(
     for (int i = 0; i < ROPE_UNITS; ++i) {
       const int u = base + 256 * i + tid;
       if (u < units) {
-        const int tok = per_tok_mul ? (int)__umulhi((uint32_t)u, per_tok_mul) : 0;
+        const int tok = TB == 1 ? 0 : per_tok_mul ? (int)__umulhi((uint32_t)u, per_tok_mul) : u;
         const int rest = u - tok * per_tok;
         const int head = groups_mul ? (int)__umulhi((uint32_t)rest, groups_mul) : rest;
         const int pair = (rest - head * groups) * V;
@@ -445,7 +446,7 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   if (tb < 1) tb = 1;
   const int64_t grid = (T + tb - 1) / tb;
   const auto mul = [](int64_t n) { return n == 1 ? 0u : (uint32_t)((1ull << 32) / n + 1); };
-  const uint32_t per_tok_mul = tb == 1 ? 0u : mul(per_tok), second = rows || staged ? mul(H) : mul(pairs / vec);
+  const uint32_t per_tok_mul = mul(per_tok), second = rows || staged ? mul(H) : mul(pairs / vec);
   if (rows) vec = 0;
   if (staged) vec = 16;
   QV_CHECK_ARG(grid <= INT32_MAX && per_tok * tb <= INT32_MAX / 2, "too many tokens or heads");

@@ -135,3 +135,35 @@ def test_rope_axes_large(gpu, dtype, D, H, sections, layout):
     edge = buf[:, ::H + 1].clone()
     E.rope_axes(x, pos, plan, out=x)
     assert torch.equal(x, want) and torch.equal(buf[:, ::H + 1], edge)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [2, 4, 8, 16])
+@pytest.mark.parametrize("T", [2047, 2048, 5000, 70001])
+def test_rope_axes_one_piece_a_token(gpu, T, D, dtype):
+    """One head whose pairs are one piece, several tokens to a workgroup: a tensor of its own, the first heads of a
+    fused buffer in place (the others stay), heads before tokens (the head stride is the whole tensor)."""
+    from qvggt_amd import awq_inference_engine as E
+    g = torch.Generator(device=gpu).manual_seed(D + T)
+    qkv = torch.randn(T, 3, D, generator=g, device=gpu).to(dtype)
+    pos = torch.randint(-100, 100000, (T, 1), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(D, (D,), device=gpu)
+    x = qkv[:, :1].contiguous()
+    out = E.rope_axes(x, pos, plan)
+    _check(out, x, pos, O.rope_pairs((D,), "block"))
+    rest = qkv[:, 1:].clone()
+    assert torch.equal(E.rope_axes(qkv[:, :1], pos, plan, out=qkv[:, :1]), out)
+    assert torch.equal(qkv[:, :1], out) and torch.equal(qkv[:, 1:], rest)
+    before = x.view(1, T, D).transpose(0, 1)
+    assert before.stride(1) == T * D
+    into = torch.zeros(1, T, D, dtype=dtype, device=gpu).transpose(0, 1)
+    assert torch.equal(E.rope_axes(before, pos, plan, out=into), out)
+
+
+@pytest.mark.parametrize("D,sections", [(64, (16, 24, 24)), (30, (2, 4)), (16, (16,))])
+def test_rope_axes_most_heads(gpu, D, sections):
+    from qvggt_amd import awq_inference_engine as E
+    g = torch.Generator(device=gpu).manual_seed(D)
+    x = torch.randn(3, 4096, D, generator=g, device=gpu).half()
+    pos = torch.randint(0, 5000, (3, len(sections)), generator=g, device=gpu, dtype=torch.int32)
+    _check(E.rope_axes(x, pos, E.rope_axes_plan(D, sections, device=gpu)), x, pos, O.rope_pairs(sections, "block"))
