@@ -140,10 +140,11 @@ struct KvUnits {
   }
 };
 
-// What the scores of a block with key scale ks are multiplied by; kept off 0 so that a masked
-// score (-inf) times it stays -inf.
+// What the scores of a block with key scale ks are multiplied by (1 for the NaN of a marked
+// block); kept off 0 so that a masked score (-inf) times it stays -inf: with a scale of 0
+// the scores, whole numbers times 16-bit queries, still come to nothing.
 __device__ __forceinline__ float kv_factor(float ks, float mul) {
-  const float c = (ks > 0.f ? ks : 1.0f) * mul;
+  const float c = (ks >= 0.f ? ks : 1.0f) * mul;
   return c < 1e-37f ? 1e-37f : c;
 }
 

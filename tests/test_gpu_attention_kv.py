@@ -438,6 +438,21 @@ def test_cached_scale_argument_and_strides(gpu):
         assert c.attention(q, scale=0.3, out=out) is out and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, F16), (64, BF16)])
+@pytest.mark.parametrize("Lq", [1, 50, 200])
+def test_cached_scale_of_zero(gpu, Lq, D, dtype):
+    """A block whose scale is 0 holds zeros, whatever its codes are (loaded ones may be anything): keys, values, both."""
+    c = _cache(gpu, 71, 1, (500,), 2, D, dtype)
+    kc, ks, vc, vs, lens = c.save_codes()
+    ks[0, 1], ks[0, 3, 0], ks[0, 7, 1] = 0, 0, 0
+    vs[0, 2], vs[0, 3, 0], vs[0, 7, 0] = 0, 0, 0
+    c.load_codes(kc, ks, vc, vs, lens)
+    assert c.k_codes[0, :, 1].any() and not c.values()[0][0, 64:128].any()
+    q = _rand(gpu, 72, 1, Lq, 4, D, dtype=dtype, sharp=3.0)
+    for causal in (False, True):
+        _check_cached(c.attention(q, causal=causal), q, c, causal)
+
+
 def test_cached_long_offsets(gpu):
     """A cache whose heads lie past 4 GB: keys of zero everywhere but in the last tokens."""
     from qvggt_amd.kv_cache import Int8KVCache
