@@ -119,9 +119,9 @@ __device__ __forceinline__ void kv_decode(const uint4& u, f16x2 f, uint4& lo, ui
 }
 
 // The scale's part of 2^ve, moving ve where the block needs it (the same in all
-// lanes).  top: the largest ve so far.  O moves with it in 32 bits: a row keeps what is
-// above some 2^-100 of the largest scale among its tile's blocks, its own or not (fp16
-// inputs span 2^40; bf16 ones could pass it).
+// lanes).  top: the largest ve so far.  O moves with it in 32 bits (KvState::follow).
+// A row keeps what is above some 2^-60 of the largest scale among the blocks that it
+// sees, whatever they weigh (fp16 inputs span 2^40; bf16 ones could pass it).
 struct KvUnits {
   int ve = 0, top = -1000;
   bool any = false;
@@ -192,6 +192,11 @@ struct KvRows {
   }
 };
 
+// What `upto`, the last key that a row sees (at least -2^28), becomes with the unit of a
+// row whose keys are behind it.
+constexpr int KV_BEHIND = -(1 << 30);
+__device__ __forceinline__ int kv_unit(int upto, int ve) { return upto < KV_BEHIND / 2 ? upto - KV_BEHIND : ve; }
+
 // Running state of 32 rows: O (dims 32 db + 8 (r / 4) + 4 h + r % 4 of the lane's row), m, l.
 template <int D>
 struct KvState {
@@ -207,6 +212,15 @@ struct KvState {
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[db][r] *= by;
+  }
+  // O from units of 2^from to 2^to, those of the values of the tile at key0.  A row that
+  // sees nothing of the tile, nor then of any behind it, stays at 2^from: far larger
+  // values, which it does not see, would take its O below what 32 bits hold (the tile's
+  // products add zeros to it).  From then on `upto`, its last key, holds that unit.
+  __device__ __forceinline__ void follow(int from, int to, int& upto, int key0) {
+    const bool sees = upto >= key0;
+    scale(__builtin_ldexpf(1.0f, sees ? from - to : 0));
+    if (!sees && upto > KV_BEHIND / 2) upto = KV_BEHIND + from;
   }
 };
 
@@ -621,7 +635,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   KvState<D> s;
   s.init();
-  int ve = 0;                                        // of O
+  int ve = 0;                                        // of the last tile's values
+  int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;    // the last key that the row sees
   if (n > 0) {
     // K of tiles 0 and 1; zero in the stage that the first PV reads (its P is zero, too)
     kt.start(klds0, wave, kraw);
@@ -652,7 +667,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       return;
     }
     qr.finish(a.scale_log2);
-    const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;                      // the last key that the row sees
     auto frag_k = [&](int stage, int f) __attribute__((always_inline)) {               // f = kb + 2 st
       if constexpr (KV8) return reinterpret_cast<const uint4*>(k_lds[stage])[((f & 1) * KS + (f >> 1)) * 64 + lane];
       else return kv_frag_k<D>(k_lds[stage], f & 1, f >> 1, h, l32);
@@ -666,10 +680,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int f = 0; f < NK; ++f) sa[f & 1] = kv_mfma<MBF>(frag_k(0, f), qr.f[f >> 1], f < 2 ? f32x16{} : sa[f & 1]);
     lds_barrier();                                   // the first K stage may be written again
-    auto rescale = [&]() __attribute__((always_inline)) {
+    // for the values of tile j
+    auto rescale = [&](int j) __attribute__((always_inline)) {
       if constexpr (KV8) {
         if (units.ve != ve) {
-          s.scale(__builtin_ldexpf(1.0f, ve - units.ve));
+          s.follow(ve, units.ve, upto, (rg.t0 + j) * KV_BLOCK);
           ve = units.ve;
         }
       }
@@ -692,7 +707,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const uint64_t seen = visible(j);
       const float kscale = ks;
       feed(j);
-      rescale();
+      rescale(j - 1);
       const float c = KV8 ? kv_factor(kscale, qr.mul) : qr.mul;
       if (j >= edge && (KV8 || seen != ~0ull)) kv_mask<2>(sc, seen & kv_below(upto - key0 + 1), h);
       kv_softmax<MBF, D, 2, true>(sc, c, s, pn, [&](int i) __attribute__((always_inline)) {
@@ -715,7 +730,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     auto last = [&](uint4 (&p)[4]) __attribute__((always_inline)) {
       clear(n - 1, before);
-      rescale();
+      rescale(n - 1);
 #pragma unroll
       for (int f = 0; f < NF; ++f) s.o[f % NV] = kv_mfma<MBF>(frag_v((n - 1) & 1, f), p[f / NV], s.o[f % NV]);
     };
@@ -733,7 +748,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   } else if (!live) {
     return;
   }
-  kv_store<BF16, D>(a, s, kv_half_sum(s.l), ve, part, row, h, row < nrows && kv_query(a, row) < rg.nq);
+  kv_store<BF16, D>(a, s, kv_half_sum(s.l), kv_unit(upto, ve), part, row, h, row < nrows && kv_query(a, row) < rg.nq);
 }
 
 // ------------------------------------------------------------------ wide form
@@ -858,7 +873,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     qr[qb].finish(a.scale_log2);
     s[qb].init();
   }
-  int ve = 0;                                        // of O
+  int ve = 0;                                        // of the last tile's values
   for (int j = 0; j < n; ++j) {
     lds_barrier();                                   // tile j is in place, stage j + 1 free
     const int buf = j & 1;
@@ -873,9 +888,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           if (seen & kv_below(upto[qb] - (rg.t0 + j) * KV_BLOCK + 1)) s[qb].l = __builtin_nanf("");
       }
       if (units.ve != ve) {
-        const float by = __builtin_ldexpf(1.0f, ve - units.ve);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) s[qb].scale(by);
+        for (int qb = 0; qb < QB; ++qb) s[qb].follow(ve, units.ve, upto[qb], (rg.t0 + j) * KV_BLOCK);
         ve = units.ve;
       }
     }
@@ -918,7 +932,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = wrow + 32 * qb + l32;
-    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), ve, part, r, h, r < nrows && kv_query(a, r) < rg.nq);
+    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), kv_unit(upto[qb], ve), part, r, h, r < nrows && kv_query(a, r) < rg.nq);
   }
 }
 
@@ -963,13 +977,13 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
   const int rc = l32 < nrows ? l32 : nrows - 1;
   const int qi = kv_query(a, rc);
   const uint16_t* qp = a.q + b * a.q_bs + qi * a.q_ts + (hk * a.G + rc - qi * a.G) * a.q_hs;
-  const int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;
+  int upto = a.causal ? rg.len - rg.nq + qi : rg.len - 1;    // the last key that the row sees
   const int first_upto = a.causal ? rg.len - rg.nq : rg.len - 1;
   KvRows<KV8, BF16, D> qr;
   KvState<D> s;
   s.init();
   KvUnits units;
-  int ve = 0;
+  int ve = 0;                                        // of the last tile's values
   if constexpr (KV8) {
     // fragments straight from memory: the next tile's K when this one's are used, its V
     // behind the last product (no spare registers: a spilled one, read back behind these
@@ -1021,7 +1035,7 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
         ks = a.ks[cache0 + tile + C::WAVES], vs = a.vs[cache0 + tile + C::WAVES];
       }
       if (units.ve != ve) {
-        s.scale(__builtin_ldexpf(1.0f, ve - units.ve));
+        s.follow(ve, units.ve, upto, key0);
         ve = units.ve;
       }
       if (seen != ~0ull || first_upto < key0 + KV_BLOCK - 1) kv_mask<KB>(sc, seen & kv_below(upto - key0 + 1), h);
@@ -1126,7 +1140,7 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
   float sum = 0.f;
 #pragma unroll
   for (int w = 0; w < C::WAVES; ++w) sum += stat[w][l32].y * __builtin_amdgcn_exp2f(stat[w][l32].x - ref);
-  const float by = sum == 0.f ? 0.f : __builtin_ldexpf(__builtin_amdgcn_exp2f(s.m - ref) / sum, ve);
+  const float by = sum == 0.f ? 0.f : __builtin_ldexpf(__builtin_amdgcn_exp2f(s.m - ref) / sum, kv_unit(upto, ve));
   float* join = reinterpret_cast<float*>(lds);       // [wave][row][D]
   if (l32 < nrows)
 #pragma unroll

@@ -453,6 +453,64 @@ def test_cached_scale_of_zero(gpu, Lq, D, dtype):
         _check_cached(c.attention(q, causal=causal), q, c, causal)
 
 
+def _check_blocks_apart(out, q, c, causal, lost=0.0):
+    """Every key of a block has the same score, so its rounded probabilities are equal and cancel; blocks that a row
+    does not look at weigh under 2^-100.  What is left are fp32 sums and the output's rounding, and what the sizes
+    in a row's sight may lose where they pass 2^60: lost times the largest value that it sees."""
+    k, v = (t[0].double().cpu().numpy() for t in c.values(int(c.lens[0])))
+    n, Lq = len(k), q.shape[1]
+    keep = np.arange(n) <= (n - Lq + np.arange(Lq))[:, None] if causal else None
+    q, got, u = q[0].double().cpu().numpy(), out[0].double().cpu().numpy(), HALF_STEP[out.dtype]
+    assert np.isfinite(got).all()
+    ref, size = (O.attention(q, k, x, q.shape[2] ** -0.5, keep) for x in (v, np.abs(v)))
+    tol = (n + 16) * 2.0 ** -24 * size + u * np.abs(ref) * 1.01 + (2.0 ** -25 if out.dtype == F16 else 0)
+    if lost:
+        tol += lost * np.where(keep, np.abs(v).max((1, 2)), 0).max(1)[:, None, None]
+    err = np.abs(got - ref)
+    assert (err <= tol).all(), (np.argwhere(err > tol)[:5], np.nanmax(err / np.maximum(tol, 1e-300)))
+
+
+def _blocks_apart(gpu, sizes, Lq, H, D, dtype, looks=True):
+    """A cache of one key head, block t's keys the unit vector t (times 30), its values of size sizes[t]; query i looks at
+    block i % blocks (some rows at none)."""
+    from qvggt_amd.kv_cache import Int8KVCache
+    nb = len(sizes)
+    n = 64 * nb - 5
+    c = Int8KVCache(1, 1, D, n, device=gpu)
+    k = torch.zeros(1, n, 1, D, device=gpu)
+    k[0, torch.arange(n), 0, torch.arange(n) // 64] = 30.0
+    v = _rand(gpu, 2, 1, n, 1, D, dtype=torch.float32) * torch.tensor(sizes, device=gpu).repeat_interleave(64)[:n].view(1, n, 1, 1)
+    c.append(k.to(dtype), v.to(dtype))
+    q = torch.zeros(1, Lq, H, D, device=gpu)
+    if looks:
+        i = torch.arange(Lq * H, device=gpu)
+        q.view(Lq * H, D)[i, i % (nb + 1)] = 30.0          # dim nb: no block's
+    return c, q.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,sizes", [
+    (BF16, (1.0, 2.0 ** -50, 8.0, 2.0 ** -55, 2.0 ** -20, 2.0 ** -50, 2.0 ** -40)),
+    (BF16, (2.0 ** -20, 2.0 ** 35, 2.0 ** -20, 2.0 ** 30, 2.0 ** -20, 1.0, 2.0 ** 35)),
+    (BF16, (2.0 ** -105, 2.0 ** -60, 2.0 ** -100, 2.0 ** -90, 2.0 ** -60, 2.0 ** -110, 2.0 ** -70)),
+    (F16, (2.0 ** -12, 2.0 ** 11, 2.0 ** -12, 1.0, 2.0 ** -12, 2.0 ** 11, 2.0 ** -3))])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Lq,H", [(9, 3), (50, 2), (300, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_cached_small_blocks_beside_large_ones(gpu, Lq, H, D, causal, dtype, sizes):
+    """Rows that look at one block keep its values whatever the size of the others within 2^60, in any order."""
+    c, q = _blocks_apart(gpu, sizes, Lq, H, D, dtype)
+    _check_blocks_apart(c.attention(q, causal=causal), q, c, causal)
+
+
+@pytest.mark.parametrize("sizes", [(1e-30, 1e30), (1e-33, 1e-11, 1e11, 1e33), (1e-33, 1e-33, 1e33, 1e33, 1e33), (1e20, 1e-10, 1e33)])
+@pytest.mark.parametrize("Lq,H", [(9, 3), (50, 2), (60, 4), (110, 1), (110, 4)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_cached_unseen_blocks_take_nothing(gpu, Lq, H, D, sizes):
+    """Causal rows that share their tiles with a much larger later block, which they do not see: nothing of theirs is lost."""
+    c, q = _blocks_apart(gpu, sizes, Lq, H, D, BF16, looks=False)
+    _check_blocks_apart(c.attention(q, causal=True), q, c, True, lost=2.0 ** -60)
+
+
 def test_cached_long_offsets(gpu):
     """A cache whose heads lie past 4 GB: keys of zero everywhere but in the last tokens."""
     from qvggt_amd.kv_cache import Int8KVCache
