@@ -126,6 +126,8 @@ class Int8KVCache:
         up to its own.  counts int32 (B,): how many of the n queries each sequence
         has; the rows of ``out`` behind them are left as they were (zero in a new
         out).  A query that sees no token gives zeros.  ``out`` must not overlap q.
+        Of the values that a query sees, what lies below 2^-60 of the largest block scale
+        among them may be lost, whatever their weights (only bfloat16 ones span so far).
         Returns (B, n, heads, head_dim)."""
         what = "Int8KVCache.attention"
         dt, scale = _kv_query(q, self.kv_heads, out, scale, what)
