@@ -438,12 +438,20 @@ __device__ __forceinline__ KvRange kv_range(const KvAttn& a, int b, int split, i
   return r;
 }
 
+// O's quotient back from units of 2^ve (16-bit values: none): a step of its own, as 2^ve
+// over a long sum is no normal number where ve comes near -120, and an exact one unless the
+// result is none.
+template <bool KV8>
+__device__ __forceinline__ float kv_out(float x, float inv, int ve) {
+  return KV8 ? __builtin_ldexpf(x * inv, ve) : x * inv;
+}
+
 // Store a lane's row: the quotient to out, or to the split's part with m and l.
-template <bool BF16, int D>
+template <bool KV8, bool BF16, int D>
 __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, float l, int ve, const KvPart& p, int row,
                                          int h, bool live) {
   if (!live) return;
-  const float inv = l == 0.f ? 0.f : __builtin_ldexpf(1.0f / l, ve);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int qi = kv_query(a, row), head = p.hk * a.G + row - qi * a.G;
   if (a.splits == 1) {
     uint16_t* op = a.out + p.b * a.o_bs + qi * a.o_ts + head * a.o_hs;
@@ -452,8 +460,8 @@ __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, f
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         uint2 w;
-        w.x = pack2<BF16>(s.o[db][4 * g] * inv, s.o[db][4 * g + 1] * inv);
-        w.y = pack2<BF16>(s.o[db][4 * g + 2] * inv, s.o[db][4 * g + 3] * inv);
+        w.x = pack2<BF16>(kv_out<KV8>(s.o[db][4 * g], inv, ve), kv_out<KV8>(s.o[db][4 * g + 1], inv, ve));
+        w.y = pack2<BF16>(kv_out<KV8>(s.o[db][4 * g + 2], inv, ve), kv_out<KV8>(s.o[db][4 * g + 3], inv, ve));
         *reinterpret_cast<uint2*>(op + 32 * db + 8 * g + 4 * h) = w;
       }
   } else {
@@ -465,7 +473,8 @@ __device__ __forceinline__ void kv_store(const KvAttn& a, const KvState<D>& s, f
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<float4*>(pp + 32 * db + 8 * g + 4 * h) =
-            make_float4(s.o[db][4 * g] * inv, s.o[db][4 * g + 1] * inv, s.o[db][4 * g + 2] * inv, s.o[db][4 * g + 3] * inv);
+            make_float4(kv_out<KV8>(s.o[db][4 * g], inv, ve), kv_out<KV8>(s.o[db][4 * g + 1], inv, ve),
+                        kv_out<KV8>(s.o[db][4 * g + 2], inv, ve), kv_out<KV8>(s.o[db][4 * g + 3], inv, ve));
     if (h == 0) a.stat[at] = make_float2(s.m, l);
   }
 }
@@ -748,7 +757,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   } else if (!live) {
     return;
   }
-  kv_store<BF16, D>(a, s, kv_half_sum(s.l), kv_unit(upto, ve), part, row, h, row < nrows && kv_query(a, row) < rg.nq);
+  kv_store<KV8, BF16, D>(a, s, kv_half_sum(s.l), kv_unit(upto, ve), part, row, h, row < nrows && kv_query(a, row) < rg.nq);
 }
 
 // ------------------------------------------------------------------ wide form
@@ -932,7 +941,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const int r = wrow + 32 * qb + l32;
-    kv_store<BF16, D>(a, s[qb], kv_half_sum(s[qb].l), kv_unit(upto[qb], ve), part, r, h, r < nrows && kv_query(a, r) < rg.nq);
+    kv_store<KV8, BF16, D>(a, s[qb], kv_half_sum(s[qb].l), kv_unit(upto[qb], ve), part, r, h, r < nrows && kv_query(a, r) < rg.nq);
   }
 }
 
@@ -1140,7 +1149,8 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
   float sum = 0.f;
 #pragma unroll
   for (int w = 0; w < C::WAVES; ++w) sum += stat[w][l32].y * __builtin_amdgcn_exp2f(stat[w][l32].x - ref);
-  const float by = sum == 0.f ? 0.f : __builtin_ldexpf(__builtin_amdgcn_exp2f(s.m - ref) / sum, kv_unit(upto, ve));
+  const float by = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(s.m - ref) / sum;
+  const int unit = kv_unit(upto, ve);
   float* join = reinterpret_cast<float*>(lds);       // [wave][row][D]
   if (l32 < nrows)
 #pragma unroll
@@ -1148,7 +1158,8 @@ __global__ __launch_bounds__(64 * kv_step_waves(KV8, D))
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<float4*>(join + (wave * 32 + l32) * D + 32 * db + 8 * g + 4 * h) =
-            make_float4(s.o[db][4 * g] * by, s.o[db][4 * g + 1] * by, s.o[db][4 * g + 2] * by, s.o[db][4 * g + 3] * by);
+            make_float4(kv_out<KV8>(s.o[db][4 * g], by, unit), kv_out<KV8>(s.o[db][4 * g + 1], by, unit),
+                        kv_out<KV8>(s.o[db][4 * g + 2], by, unit), kv_out<KV8>(s.o[db][4 * g + 3], by, unit));
   __syncthreads();
   const int rows_out = nrows < rg.nq * a.G ? nrows : rg.nq * a.G;
   for (int i = tid; i < rows_out * (D / 4); i += 64 * C::WAVES) {

@@ -511,6 +511,26 @@ def test_cached_unseen_blocks_take_nothing(gpu, Lq, H, D, sizes):
     _check_blocks_apart(c.attention(q, causal=True), q, c, True, lost=2.0 ** -60)
 
 
+@pytest.mark.parametrize("Lq,H", [(1, 2), (50, 1), (200, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("split", [False, True])
+def test_cached_tiny_values_of_many_tokens(gpu, Lq, H, D, split):
+    """The smallest scale beside a sum of 8000 weights of 2^14.5: their quotient is no normal number, the result is.
+    One value for all tokens comes back exactly (8000 terms at 2^-23 are under half a step)."""
+    from qvggt_amd.kv_cache import Int8KVCache
+    n = 8000
+    c = Int8KVCache(1, 1, D, n, device=gpu)
+    k, v = torch.zeros(1, n, 1, D, device=gpu), torch.full((1, n, 1, D), 2.0 ** -114, device=gpu)
+    k[0, 64:, 0, 0] = 1.0
+    c.append(k.bfloat16(), v.bfloat16())
+    assert (c.v_scales[0, 0, :-(-n // 64)] == 2.0 ** -120).all()
+    q = torch.zeros(1, Lq, H, D, device=gpu)
+    q[..., 0] = 7.5 * math.log(2.0) * D ** 0.5
+    if not split:
+        c._bound = 0                                      # the hint only
+    assert (c.attention(q.bfloat16()) == 2.0 ** -114).all()
+
+
 def test_cached_long_offsets(gpu):
     """A cache whose heads lie past 4 GB: keys of zero everywhere but in the last tokens."""
     from qvggt_amd.kv_cache import Int8KVCache
