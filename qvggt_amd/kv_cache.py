@@ -91,8 +91,10 @@ class Int8KVCache:
                       _ptr(self.v_scales), _ptr(self.lens if start is None else start), _ptr(self.lens),
                       _ptr(self._tickets), _ptr(counts), self.batch, n, self.kv_heads, self.head_dim, self.blocks,
                       _kv_strides(k), _kv_strides(v), _stream(dev))
-        # how long a sequence may be by now: a hint for the attention's split of the keys
-        self._bound = min(self.capacity, self._bound + n)
+        # how long a sequence may be by now: a hint for the attention's split of the keys.  Behind a
+        # start, which lies on the GPU, a sequence may have any length.
+        own = start is None or start.data_ptr() == self.lens.data_ptr()
+        self._bound = min(self.capacity, self._bound + n) if own else self.capacity
 
     def values(self, n: int | None = None, first: torch.Tensor | None = None, dtype: torch.dtype = torch.float32):
         """The cached (keys, values) of n tokens (default: the capacity) of each sequence
@@ -118,7 +120,8 @@ class Int8KVCache:
 
     # ------------------------------------------------------------ attention
     def attention(self, q: torch.Tensor, scale: float | None = None, causal: bool = False,
-                  counts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                  counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  longest: int | None = None) -> torch.Tensor:
         """Attention of q (B, n, heads, head_dim), fp16 or bf16, over the cached tokens of
         each sequence; heads a multiple of kv_heads, scale head_dim**-0.5 by default.
 
@@ -126,6 +129,11 @@ class Int8KVCache:
         up to its own.  counts int32 (B,): how many of the n queries each sequence
         has; the rows of ``out`` behind them are left as they were (zero in a new
         out).  A query that sees no token gives zeros.  ``out`` must not overlap q.
+        longest: about how many tokens the longest sequence has, for the split of the
+        keys over the chip, and for nothing else: any number gives the result.  By
+        default the tokens of the calls to ``append`` so far (those of a graph's capture,
+        not of its replays), the capacity once one had a ``start``: a program that goes
+        back and forth in a large cache, or replays, does well to say it.
         Of the values that a query sees, what lies below 2^-60 of the largest block scale
         among them may be lost, whatever their weights (only bfloat16 ones span so far).
         Returns (B, n, heads, head_dim)."""
@@ -135,17 +143,20 @@ class Int8KVCache:
         if B != self.batch or D != self.head_dim:
             _fail(f"{what}: q must be ({self.batch}, n, heads, {self.head_dim}), got {tuple(q.shape)}")
         self._per_sequence(counts, what, "counts")
+        if longest is not None and longest < 0:
+            _fail(f"{what}: longest must not be negative, got {longest}")
+        keys = self._bound if longest is None else min(self.capacity, int(longest))
         dev = _on_gpu(q, counts, out, self.lens, what=what)
         q = _kv_rows(q)
         if out is None:
             new = torch.empty if counts is None else torch.zeros
             out = new((B, n, H, D), dtype=q.dtype, device=q.device)
-        ws_bytes = _kv_workspace_bytes(1, B, n, H, self.kv_heads, D, self._bound)
+        ws_bytes = _kv_workspace_bytes(1, B, n, H, self.kv_heads, D, keys)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
         with _device(dev):
             _lib.call("qv_kv8_attention", _ptr(q), _ptr(out), dt, _ptr(self.k_codes), _ptr(self.v_codes), _ptr(self.k_scales),
                       _ptr(self.v_scales), _ptr(self.lens), _ptr(counts), 1 if causal else 0, B, n, H, self.kv_heads, D,
-                      self.blocks, self._bound, _kv_strides(q), _kv_strides(out), scale, _ptr(ws), ws_bytes, _stream(dev))
+                      self.blocks, keys, _kv_strides(q), _kv_strides(out), scale, _ptr(ws), ws_bytes, _stream(dev))
         return out
 
     # ----------------------------------------------- codes in token order

@@ -162,6 +162,45 @@ def test_attention_kv_refusals():
             c.attention(*args, **kw)
 
 
+def test_cache_length_hint(monkeypatch):
+    """How many keys the attention's split is laid out for: the tokens appended so far, the capacity once a start was
+    given (it lies on the GPU and may be anything), or what the caller says.  No kernel runs here."""
+    import contextlib
+
+    from qvggt_amd import kv_cache as M
+    calls = []
+    monkeypatch.setattr(M, "_on_gpu", lambda *t, what: 0)
+    monkeypatch.setattr(M, "_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(M, "_stream", lambda dev: 0)
+    monkeypatch.setattr(M._lib, "call", lambda name, *args: calls.append((name, args)))
+    c = Int8KVCache(1, 1, 64, 1 << 20, device="cpu")
+    q, k = torch.zeros(1, 1, 4, 64).half(), torch.zeros(1, 100, 1, 64).half()
+    at = torch.tensor([(1 << 20) - 100], dtype=torch.int32)
+
+    def keys(**kw):
+        c.attention(q, **kw)
+        name, args = calls[-1]
+        assert name == "qv_kv8_attention"
+        assert args[-2] == E._kv_workspace_bytes(1, 1, 1, 4, 1, 64, args[16])     # the workspace of the same plan
+        return args[16]
+
+    assert keys() == 0 and keys(longest=5000) == 5000
+    c.append(k, k)
+    assert keys() == 100 and keys(longest=0) == 0 and keys(longest=1 << 30) == 1 << 20
+    c.append(k, k, start=c.lens)                           # its own lengths
+    assert keys() == 200
+    c.append(k, k, start=at)                               # far behind them: one split would walk 16384 blocks
+    assert keys() == 1 << 20
+    c.reset()
+    assert keys() == 0
+    c.append(k, k)
+    for _ in range(5):                                     # back and forth: not 100 more each time
+        c.append(k, k, start=at)
+        assert keys() == 1 << 20 and keys(longest=300) == 300
+    with pytest.raises(RuntimeError, match="longest"):
+        c.attention(q, longest=-1)
+
+
 def test_c_entries_refuse():
     """Bad arguments end at the C entries with a message, before any device work (pointers here are never followed)."""
     import ctypes as C
