@@ -15,6 +15,7 @@ from .awq_inference_engine import (_device, _dtype_code, _fail, _kv_query, _kv_r
                                    _on_gpu, _ptr, _stream)
 
 BLOCK = 64   # tokens of a block
+MOST_BLOCKS = (1 << 23) - 1   # of a sequence, as the C entries count them
 
 
 class Int8KVCache:
@@ -39,7 +40,7 @@ class Int8KVCache:
         what = "Int8KVCache"
         if head_dim not in (64, 128):
             _fail(f"{what}: head_dim must be 64 or 128, got {head_dim}")
-        if not (1 <= batch <= 32767 and 1 <= kv_heads <= 65535 and 1 <= capacity <= 64 << 23):
+        if not (1 <= batch <= 32767 and 1 <= kv_heads <= 65535 and 1 <= capacity <= MOST_BLOCKS * BLOCK):
             _fail(f"{what}: bad batch {batch}, kv_heads {kv_heads} or capacity {capacity}")
         self.batch, self.kv_heads, self.head_dim = batch, kv_heads, head_dim
         self.blocks = -(-capacity // BLOCK)
@@ -103,7 +104,7 @@ class Int8KVCache:
         largest lies between 2^-14 and 2^15 (a value may come back half a step larger)."""
         what = "Int8KVCache.values"
         n = self.capacity if n is None else n
-        if not 0 <= n <= 64 << 23:
+        if not 0 <= n < 1 << 29:
             _fail(f"{what}: bad number of tokens {n}")
         if dtype not in (torch.float32, torch.float16, torch.bfloat16):
             _fail(f"{what}: dtype must be float32, float16 or bfloat16, got {dtype}")

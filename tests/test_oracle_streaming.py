@@ -124,6 +124,27 @@ def test_cache_refusals():
             c.values(**kw)
 
 
+def test_cache_limits_are_those_of_the_c_entries():
+    """The largest capacity and range pass both sides; one block or token more is refused before anything is allocated."""
+    from qvggt_amd import _lib
+    most = (1 << 29) - 64
+    c = Int8KVCache(1, 1, 64, most, device="meta")
+    assert c.capacity == most and c.blocks == (1 << 23) - 1
+    for capacity in (most + 1, 1 << 29):
+        with pytest.raises(RuntimeError, match="bad batch"):
+            Int8KVCache(1, 1, 64, capacity, device="meta")
+    with pytest.raises(RuntimeError, match="number of tokens"):
+        c.values(1 << 29)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        c.values((1 << 29) - 1)
+    lib, p = _lib.load(), 1 << 20
+    val = lambda n, blocks: lib.qv_kv8_values(p, p, p, p, p, None, None, p, 2, 1, n, 1, 64, blocks, None)
+    said = lambda: lib.qv_last_error().decode()
+    assert val(5, 1 << 23) == -1 and "cache shape" in said() and val(1 << 29, 3) == -1 and "number of tokens" in said()
+    # what Python lets through comes to the next check, the null output
+    assert val((1 << 29) - 1, c.blocks) == -1 and "null" in said()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_cache_block_order_is_a_permutation(D):
     key, val = Int8KVCache(1, 1, D, 64, device="cpu")._order()
