@@ -1232,9 +1232,13 @@ static KvPlan kv_plan(bool kv8, int64_t B, int64_t Lq, int64_t H, int64_t Hk, in
     p.step = true, p.qb = 1, p.row_tiles = 1;
     // 8-bit: two workgroups a CU, twice as many splits where sequences may differ (16 of up
     // to 8001 tokens: as fast when all are full, 19 instead of 27 us when all hold 2048).
-    // 16-bit: one a CU, and from half the CUs on no split, which saves the join (8 x 16 heads
-    // over 1374 keys: 11.3 us; split in two 12.3 and 3.9)
-    const int64_t slots = kv8 ? (B > 1 ? 1024 : 512) : heads >= 128 ? 1 : 256;
+    // 16-bit: one a CU; from half the CUs on no split, which saves the join, while keys and
+    // values fit the 256 MB that the caches behind the L2 hold: 8 x 16 heads of 64 over 1374
+    // keys 14.5 us against 18.5 split in two, 6870 keys (225 MB) 37.7 against 40.5; but 10992
+    // 93.9 against 72.2 and 43968 365 against 280, as half the CUs do not draw what the HBM
+    // gives (heads of 128: 1374 keys 20.9 and 21.0, 13740 187 against 158)
+    const bool kept = 4 * heads * keys * D <= (256 << 20);
+    const int64_t slots = kv8 ? (B > 1 ? 1024 : 512) : heads >= 128 && kept ? 1 : 256;
     int64_t s = heads < slots ? slots / (heads > 0 ? heads : 1) : 1;
     if (s > tiles / 8) s = tiles / 8;                       // a tile or two for each wave at least
     if (s > 64) s = 64;

@@ -150,6 +150,21 @@ def test_cross_split_keys(gpu, Lq, Lk, H, Hk, D, dtype):
     assert not E.cross_attention(q, k, v, key_mask=keep & False).any()
 
 
+@pytest.mark.parametrize("B,H,Lk,D", [(8, 16, 9001, 64), (2, 64, 5003, 128)])
+def test_cross_split_keys_of_many_heads(gpu, B, H, Lk, D):
+    """One query of 128 heads over more keys than the caches hold: split in two, lengths of all kinds."""
+    from qvggt_amd import awq_inference_engine as E
+    assert E._kv_workspace_bytes(0, B, 1, H, H, D, Lk) > 0
+    q, k, v = _qkv(gpu, 27, B, 1, Lk, H, H, D, F16, 3.0)
+    out = E.cross_attention(q, k, v)
+    for b in (0, B - 1):
+        _close(out[b], q[b], k[b], v[b])
+    lens = torch.tensor([(1, Lk // 2, Lk // 2 + 70, 0, Lk, 64, 65, 5000)[b] for b in range(B)], dtype=torch.int32, device=gpu)
+    out = E.cross_attention(q, k, v, kv_lens=lens)
+    for b, n in enumerate(lens.tolist()):
+        _close(out[b], q[b], k[b, :n], v[b, :n])
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("B,Lq,Lk", [(1, 1, 1374), (3, 40, 300), (1, 300, 1374), (1, 1374, 1374)])
 def test_cross_weights_sum_to_one(gpu, B, Lq, Lk, dtype):

@@ -145,6 +145,18 @@ def test_cache_limits_are_those_of_the_c_entries():
     assert val((1 << 29) - 1, c.blocks) == -1 and "null" in said()
 
 
+def test_cross_split_of_many_heads():
+    """One query, 128 to 255 heads: no split while the keys and values stay in the caches (256 MB), two behind that;
+    from a head for each CU on never."""
+    part = lambda heads, D: heads * (4 * D + 8)
+    need = lambda heads, D, keys: E._kv_workspace_bytes(0, heads, 1, 1, 1, D, keys)
+    for D in (64, 128):
+        fits = (256 << 20) // (4 * 128 * D)
+        assert need(128, D, 1374) == need(128, D, fits) == need(256, D, 40000) == 0
+        assert need(128, D, fits + 1) == need(128, D, 43968) == 2 * part(128, D)
+        assert need(120, D, 1374) == 2 * part(120, D)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_cache_block_order_is_a_permutation(D):
     key, val = Int8KVCache(1, 1, D, 64, device="cpu")._order()
