@@ -165,7 +165,8 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(
   }
 }
 
-// The same for heads of 64 to 512 dims (a power of two) with chunks in multiples of 4: a
+// The same for large tensors of 8 and more heads of 64 to 512 dims (a power of two) with chunks
+// in multiples of 4 (the rule with both sides stands at the entry): a
 // lane takes 8 consecutive dims, so that rows are read and written whole, and reads the
 // partners of each 4 of them a second time (from the L1).  A row lies within one wave,
 // whose loads all come before its stores: x and out may be the same.  43968 tokens of 32
@@ -427,16 +428,24 @@ extern "C" int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* 
   }
   QV_CHECK_ARG((uintptr_t)x % es == 0 && (uintptr_t)out % es == 0, "x and out must be aligned to their type");
   const int pairs = (int)(D / 2);
-  // whole rows: 8 dims a lane, rows within a wave, and enough of them that bytes count.  T x 32
-  // heads of 64 fp16 dims: with chunks in fours 65 us at 43968 tokens, in pieces 70, but 6.4 and
-  // 5.5 at 1374; with pieces of 1 or 2 dims staged in LDS 72, in pieces 132 and 94 (10992 tokens:
-  // 20, in pieces 27 and 21; 344 tokens: 6.0, in pieces 5.1 and 4.3).  32-bit types gain nothing
-  // by the stage (146, in pieces of 1 152, of 2 142 against 138).
+  // whole rows: 8 dims a lane, rows within a wave; from where bytes count, and for 8 heads and
+  // more, as fewer leave a workgroup bound by its sines (one head of 64 fp16 dims, 200 MB: pieces
+  // of 4 dims 78 us, rows 112; of 1 dim 104, staged 156; 4 heads 37 and 41; 65 and 50).  In us, by
+  // bytes read and written:
+  //  * 16-bit pieces of 4 dims, 32 heads: 360 MB 71 and 68, 80 MB 16.9 and 16.0, 6 MB 5.5 and 6.4;
+  //  * pieces of 8 dims are whole 16 bytes as they are: 360 MB 71.5 and 67.3 (fp32 80 and 74), but
+  //    80 MB 13.7 and 15.4 (fp32 15.1 and 16.6); fp32 pieces of 4: 360 MB 71 and 74;
+  //  * 16-bit pieces of 1 or 2 dims, staged in LDS: 128 MB 40 and 28 against 26, 60 MB 22 and 16.6
+  //    against 16, 16 MB 8.7 and 6.7 against 7.5, 4 MB 4.8 and 4.1 against 5.5 (the 64 MB of the
+  //    rows are late for pieces of 1).  32-bit types gain nothing by the stage (360 MB: 146, in
+  //    pieces of 1 152, of 2 142).
   const int wide = 8 * es < 16 ? 8 * es : 16;
-  const bool whole = 2 * T * H * D * es > (64 << 20) && D >= 64 && D <= 512 && (D & (D - 1)) == 0 &&
+  const int64_t bytes = 2 * T * H * D * es;
+  const bool whole = bytes > (64 << 20) && H >= 8 && D >= 64 && D <= 512 && (D & (D - 1)) == 0 &&
                      x_token_stride % 8 == 0 && x_head_stride % 8 == 0 && out_token_stride % 8 == 0 &&
                      out_head_stride % 8 == 0 && (uintptr_t)x % wide == 0 && (uintptr_t)out % wide == 0;
-  const bool rows = whole && vec >= 4, staged = whole && vec < 4 && es == 2;
+  const bool rows = whole && (vec == 8 ? bytes > (256 << 20) : vec == 4 && es == 2);
+  const bool staged = whole && vec < 4 && es == 2;
   const int64_t per_tok = rows || staged ? H * (D / 8) : H * (pairs / vec);
   // tokens of a workgroup: one round of pieces (1024), at most the table, and
   // enough workgroups to fill the chip

@@ -167,3 +167,31 @@ def test_rope_axes_most_heads(gpu, D, sections):
     x = torch.randn(3, 4096, D, generator=g, device=gpu).half()
     pos = torch.randint(0, 5000, (3, len(sections)), generator=g, device=gpu, dtype=torch.int32)
     _check(E.rope_axes(x, pos, E.rope_axes_plan(D, sections, device=gpu)), x, pos, O.rope_pairs(sections, "block"))
+
+
+@pytest.mark.parametrize("dtype,D,H,sections,layout,mb", [(torch.float16, 64, 8, (32, 32), "block", 260),
+                                                          (torch.bfloat16, 128, 24, (128,), "half", 260),
+                                                          (torch.float32, 64, 9, (32, 32), "half", 260),
+                                                          (torch.float16, 128, 8, (64, 64), "block", 66),
+                                                          (torch.float32, 64, 8, (16, 24, 24), "block", 66),
+                                                          (torch.float16, 256, 8, (8, 64), "block", 66),
+                                                          (torch.bfloat16, 512, 9, (8, 504), "half", 66),
+                                                          (torch.float16, 512, 8, (510,), "block", 66),
+                                                          (torch.bfloat16, 256, 8, (6, 250), "half", 66),
+                                                          (torch.float16, 64, 7, (10, 26, 28), "block", 66),
+                                                          (torch.float16, 64, 7, (16, 24, 24), "block", 66)])
+def test_rope_axes_large_by_heads_and_pieces(gpu, dtype, D, H, sections, layout, mb):
+    """Both sides of the rule that takes whole rows (heads, bytes, width of the pieces): the bits of the same tokens in
+    small calls, inside a fused buffer and in place."""
+    from qvggt_amd import awq_inference_engine as E
+    T = (mb << 20) // (2 * H * D * torch.empty(0, dtype=dtype).element_size()) + 37
+    g = torch.Generator(device=gpu).manual_seed(D + H)
+    buf = torch.randn(T, H + 1, D, generator=g, device=gpu).to(dtype)
+    x, edge = buf[:, 1:], buf[:, 0].clone()
+    pos = torch.randint(-100, 100000, (T, len(sections)), generator=g, device=gpu, dtype=torch.int32)
+    plan = E.rope_axes_plan(D, sections, layout=layout, device=gpu)
+    want = torch.cat([E.rope_axes(x[i:i + 1500], pos[i:i + 1500], plan) for i in range(0, T, 1500)])
+    _check(want[-50:], x[-50:], pos[-50:], O.rope_pairs(sections, layout))
+    assert torch.equal(E.rope_axes(x, pos, plan), want)
+    E.rope_axes(x, pos, plan, out=x)
+    assert torch.equal(x, want) and torch.equal(buf[:, 0], edge)
