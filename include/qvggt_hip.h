@@ -354,8 +354,9 @@ int qv_rope_axes(const void* x, void* out, int dtype, const int32_t* positions,
  * and head strides in elements, multiples of 8; dims contiguous.
  * Sequence b gets its first counts[b] tokens (NULL: n) behind start[b] cached ones
  * (what it held behind them is dropped, what does not fit is left out), and lens[b] is
- * set to their number; start may be lens itself.  tickets: B * (Hk + 1) *
- * QV_KV8_TICKETS words, 0 at the first call, kept with the cache.  A block's scale is the smallest number of four
+ * set to their number; start may be lens itself.  Where start passes lens the tokens in
+ * between are what the blocks hold there.  tickets: B * (Hk + 1) * QV_KV8_TICKETS words, 0
+ * at the first call, kept with the cache.  A block's scale is the smallest number of four
  * significant bits that is at least amax / 127 over its new tokens, or the one it had
  * where that is larger; value = code * scale, code = rint(x / scale), ties to even; the
  * old codes of a block whose scale grows are rounded again.  A NaN or infinity
@@ -401,7 +402,8 @@ int qv_attention_cross(const void* q, const void* k, const void* v, void* out, i
  * The same over the cache of qv_kv8_append, keys 0 .. lens[b] - 1.  counts (B; NULL: Lq):
  * queries of each sequence; the rows of out behind them are left as they were.
  * causal: the queries are the last counts[b] tokens, each sees the keys up to its
- * own.  keys: tokens that a sequence may hold, for the split only.
+ * own.  keys: tokens that a sequence may hold, for the split only.  Of the values that a
+ * query sees, what lies below 2^-60 of the largest block scale among them may be lost.
  */
 int qv_kv8_attention(const void* q, void* out, int dtype, const void* k_codes,
                      const void* v_codes, const float* k_scales, const float* v_scales,

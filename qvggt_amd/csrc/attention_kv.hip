@@ -23,7 +23,8 @@
 //
 // 8-bit values: scores are products of 16-bit queries with whole numbers, the key
 // block's scale goes into c.  bf16 queries become fp16 under a power of two of their
-// row (exact down to 2^-38 of the row's largest).  Value codes are multiplied by
+// row, its largest at 2^13 to 2^14: exact down to 2^-30 of that one's power of two, what is
+// smaller off by at most 2^-38 of it (half of fp16's last step).  Value codes are multiplied by
 // their scale over a power of two 2^ve that all of O carries: exact in fp16, as a
 // scale has four significant bits; ve moves (and O with it) only when a block's
 // scale leaves 2^(ve - 16) .. 2^(ve + 4).

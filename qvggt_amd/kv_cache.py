@@ -30,10 +30,11 @@ class Int8KVCache:
     filled by several calls keeps the largest scale that it needed, and its
     earlier codes are rounded again when that grows.
 
-    ``lens`` (int32, on the GPU) holds the tokens of each sequence.  Calls only
-    enqueue work, in stream order, and can be captured into graphs: a replayed
-    ``append`` goes on from the ``lens`` that it finds.  One cache is written by
-    one stream at a time.
+    ``lens`` (int32, on the GPU) holds the tokens of each sequence.  ``append``,
+    ``values``, ``attention`` and ``reset`` only enqueue work, in stream order, and can
+    be captured into graphs: a replayed ``append`` goes on from the ``lens`` that it
+    finds.  ``load_codes`` and ``save_codes`` wait for the GPU.  One cache is written
+    by one stream at a time.
     """
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, capacity: int, device="cuda"):
@@ -57,7 +58,7 @@ class Int8KVCache:
 
     # ------------------------------------------------------------- contents
     def reset(self) -> None:
-        """Forget all tokens."""
+        """Forget all tokens (``lens`` becomes 0; the blocks are written anew as they fill)."""
         self.lens.zero_()
         self._bound = 0
 
@@ -71,8 +72,10 @@ class Int8KVCache:
 
         counts (B,) int32: how many of the n tokens each sequence has (the rest is
         padding; not read).  start (B,) int32: append behind that many tokens in
-        place of ``lens``; what the sequence held behind them is dropped.  Tokens
-        past the capacity are dropped (``lens`` stops there)."""
+        place of ``lens``; what the sequence held behind them is dropped.  Where start
+        passes ``lens`` the tokens in between are what the blocks hold there: zeros in a
+        new cache, or what was dropped or forgotten.  Tokens past the capacity are
+        dropped (``lens`` stops there)."""
         what = "Int8KVCache.append"
         dt = _dtype_code(k, what)
         want = (self.batch, self.kv_heads, self.head_dim)
