@@ -539,12 +539,14 @@ struct KvTiles {
 // j - 1, a few of each in every slot, so that no product stands alone.  K is in LDS two
 // tiles ahead, V comes with its own tile, and the workgroup meets once a tile.
 // Bound by issue: a wave's tile of D = 128 is 32 MFMAs and 32 exponentials with their
-// multiply-adds, conversions and sums, and an MFMA takes 10 to 18 cycles of vector
-// issue too.  Two workgroups a CU need 2.1 us a tile, one alone 1.24: with the chip full
-// 1050 TF/s over 16-bit and 950 over 8-bit keys (a large fp16 matrix product of the
-// library: 1170).  64 rows a wave would halve the LDS reads, but at D = 128 O and the queries leave no registers for it: with O in
-// accumulation registers 1374 queries of 16 heads took 112 us instead of 87.  For 33 to
-// 128 rows of D = 64 half of a wide workgroup's rows would be empty.
+// multiply-adds, conversions and sums, 112 vector instructions beside the MFMAs over 16-bit
+// keys and 230 over 8-bit ones.  4096 queries of 16 heads over 10992 keys, two workgroups on
+// each CU: 1007 and 918 TF/s (a large fp16 matrix product of the library: 1170), 2.1 and 2.3
+// us a tile (one workgroup alone 1.24 and 1.55); there a wave issues in 38 and 41 % of its
+// cycles, is ready but held in 40 and 38 %, and the matrix pipe is busy in 47 and 38 %.
+// 64 rows a wave would halve the LDS reads, but at D = 128 O and the queries leave no
+// registers for it: with O in accumulation registers 1374 queries of 16 heads took 112 us
+// instead of 87.  For 33 to 128 rows of D = 64 half of a wide workgroup's rows would be empty.
 template <bool KV8, bool BF16, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_pipe_kernel(const KvAttn a) {
   constexpr bool MBF = BF16 && !KV8;
@@ -766,10 +768,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // every code that is decoded serves twice the rows.  Inside a tile the second block's QK
 // runs beside the first one's softmax, the first one's PV beside the second's.
 // Bound by issue: 64 x 64 scores a tile and wave cost 32 MFMAs and 64 exponentials of 8
-// cycles with their multiply-adds, conversions and sums.  Two workgroups a CU need 2.43 us a
-// tile, one alone 1.48: 890 TF/s over 16-bit keys and 850 over the cache with the chip full.
-// 1374 queries of 16 heads over 10992 keys: 91 us and 7 of join under a trace (90 in all
-// without); over a cache of 43968 tokens 349 and 7 (323 in all without).
+// cycles with their multiply-adds, conversions and sums, 221 vector instructions beside the
+// MFMAs over 16-bit keys and 286 over the cache (attention.hip, whose queries carry the
+// scale: 177).  8192 queries of 16 heads over 10992 keys, two workgroups on each CU: 940 and
+// 854 TF/s, 2.24 and 2.47 us a tile (one alone 1.36 and 1.54); a wave issues in 47 and 45 %
+// of its cycles, is ready but held in 38 and 35 %, the matrix pipe is busy in 43 and 37 %.
+// 1374 queries of 16 heads over 10992 keys: 92 us and 7 of join under a trace (86 to 90 in
+// all without); over a cache of 43968 tokens 352 and 7 (311 to 323 in all without).
 template <bool KV8, bool BF16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv_attn_wide_kernel(const KvAttn a) {
   constexpr int D = 64, QB = 2;
@@ -948,8 +953,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // ------------------------------------------------------------------ step form
 // Bound by the bytes of the keys and values: 16 sequences of 8000 cached tokens, 8 heads of
-// 128 dims, read at 6.2 TB/s (a large copy moves 5.2, a read alone more).  16-bit D = 64 takes 8
-// waves: 8 x 16 heads over 1374 keys 11.3 us, 4.0 TB/s.  A wave has tiles of its own,
+// 128 dims, 43 us, 6.1 TB/s (a large copy moves 5.2, a read alone more).  16-bit D = 64 takes 8
+// waves: 8 x 16 heads over 1374 keys 11.1 us, 4.0 TB/s.  A wave has tiles of its own,
 // so that none waits for another before the end; 32 rows fill the MFMA's columns however few
 // there are, and cost nothing that the bytes would not.
 constexpr int kv_step_waves(bool kv8, int d) { return !kv8 && d == 64 ? 8 : 4; }
@@ -1251,8 +1256,11 @@ static KvPlan kv_plan(bool kv8, int64_t B, int64_t Lq, int64_t H, int64_t Hk, in
   const int64_t wg = heads * p.row_tiles;
   // time of s splits in ns: rounds of 512 workgroups, two a CU (the last cheaper with at
   // most one a CU), each of its tiles and some 3 tiles' worth of prologue and end; the
-  // join.  Several sequences may be of any lengths: the mean of all full, and of half the
-  // keys spread over the CUs with one sequence still full.
+  // join.  A tile's time lies between those over 16- and 8-bit keys (two a CU: wide 2243 and
+  // 2468, D = 128 2092 and 2297; one: 1358 and 1543, 1239 and 1553; few rows of D = 64 1182
+  // and 806 over keys that stay in the caches, 1665 and 993 over ones that do not).
+  // Several sequences may be of any lengths: the mean of all full, and of half the keys
+  // spread over the CUs with one sequence still full.
   const double pair = p.qb == 2 ? 2430 : D == 64 ? 1300 : 2100, one = p.qb == 2 ? 1480 : D == 64 ? 860 : 1240;
   double best = 1e300;
   p.splits = 1;

@@ -15,8 +15,8 @@
 // pieces of x (V dims at lo, V at hi; 16 bytes each where sections and strides
 // allow it), compute one sine and cosine per (token, pair) into LDS while those
 // loads are in flight, and apply them to every head.  Bound by the bytes of x,
-// read once and written once.  16 tokens of 24 heads of 128 dims: 3.4 us, the launch and
-// two dependent reads; 1374 of 32 heads of 64: 5.5 us, 2.1 TB/s; 43968 of them: 65 us, 5.6 TB/s.
+// read once and written once.  16 tokens of 24 heads of 128 dims: 3.5 us, the launch and
+// two dependent reads; 1374 of 32 heads of 64: 5.3 us, 2.1 TB/s; 43968 of them: 65 us, 5.6 TB/s.
 #include "common.h"
 
 namespace qv {
