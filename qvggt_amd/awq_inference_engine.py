@@ -815,7 +815,8 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, plan: RopeAxesPlan, out:
             _fail(f"{what}: out must be {x.dtype} {tuple(x.shape)} with unit dim stride")
         if _overlaps_itself(out):
             _fail(f"{what}: out must not overlap itself")
-        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
+        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride() and x.numel() and any(
+                a != b for a, b, n in zip(out.stride(), x.stride(), x.shape) if n > 1):
             _fail(f"{what}: in place, out must be x")
     dev = _on_gpu(x, positions, plan.turns, out, what=what)
     if x.stride(2) != 1:

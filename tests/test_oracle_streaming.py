@@ -101,6 +101,20 @@ def test_rope_axes_refusals():
             E.rope_axes(*args)
 
 
+def test_rope_axes_in_place_of_one_or_no_token():
+    """The stride of a dim of one or none says nothing: a view of the same token, empty tensors of any strides are taken."""
+    plan = E.rope_axes_plan(64, (32, 32))
+    qkv = torch.zeros(4, 9, 64, dtype=torch.float16)
+    one = qkv[:1, :3]
+    for x, out in ((one, qkv.view(-1)[:192].view(1, 3, 64)),
+                   (qkv[:, :1][:1], qkv.view(-1)[:64].view(1, 1, 64)), (qkv[:0, :3], torch.empty(0, 3, 64, dtype=torch.float16))):
+        assert x.data_ptr() == out.data_ptr() and x.stride() != out.stride()
+        with pytest.raises(RuntimeError, match="GPU only"):
+            E.rope_axes(x, torch.zeros(len(x), 2, dtype=torch.int32), plan, out)
+    with pytest.raises(RuntimeError, match="in place"):
+        E.rope_axes(qkv[:2, :3], torch.zeros(2, 2, dtype=torch.int32), plan, qkv.view(-1)[:384].view(2, 3, 64))
+
+
 def test_cache_refusals():
     for bad in (dict(batch=0, kv_heads=1, head_dim=64, capacity=1), dict(batch=1, kv_heads=0, head_dim=64, capacity=1),
                 dict(batch=1, kv_heads=1, head_dim=96, capacity=1), dict(batch=1, kv_heads=1, head_dim=64, capacity=0)):
