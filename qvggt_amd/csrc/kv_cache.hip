@@ -12,12 +12,12 @@
 // A NaN or infinity makes the scale of its (block, head) NaN, and stays until the
 // block is begun again: the cache does not hide it.
 //
-// Both kernels are bound by bytes: the new values read once, the codes written once
-// (append), codes read and values written once (values).  A prompt of up to 2900 tokens
-// for each of 8 sequences, 8 heads of 128 fp16 dims: append 25 us, values to float32 30 us
-// (half full: 2.9 and 4.0 TB/s; the length of the longest sequence counts).  One token
-// for each of 32 sequences: append 6.4 us, launch and three dependent reads; 64 tokens
-// of each as float32: 9.0 us, 21 MB.
+// Both move the new values once and the codes once (append), codes and values once (values).
+// A prompt of up to 2900 tokens for each of 8 sequences, half full, 8 heads of 128 fp16 dims:
+// append 25.5 us for 72 MB, 2.9 TB/s, as the loads, codes and stores of a block take turns
+// behind three barriers; values to float32 30 us for 217 MB, the zeros behind the lengths
+// among them.  One token for each of 32 sequences: append 6.3 us, launch and three dependent
+// reads; 64 tokens of each as float32: 9.2 us, 21 MB.
 #include "kv_cache.h"
 
 namespace qv {
