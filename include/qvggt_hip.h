@@ -448,8 +448,8 @@ int qv_packed_attention(const void* q, const void* k, const void* v, void* out, 
  * Append k, v (B, n, Hk, D): counts[b] tokens (NULL: n) of each sequence behind start[b]; or, with
  * cu (B + 1), k, v (T, Hk, D): tokens cu[b] .. cu[b + 1] - 1, at most n of a sequence expected.
  * lens[b] becomes their number, what passes the capacity is dropped; start may be lens itself.
- * Weights of new tokens (those between lens and start among them) are 0, positions slot +
- * evicted[b].  tickets: B * QV_PAGED_TICKETS words,
+ * Weights of new tokens become 0, their positions slot + evicted[b]; those of slots in front of
+ * start (also between lens and it) stay as they are.  tickets: B * QV_PAGED_TICKETS words,
  * 0 at the first call, kept with the cache.  Strides: batch, token, head, multiples of 8.
  */
 #define QV_PAGED_TICKETS 32

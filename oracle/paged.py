@@ -63,9 +63,8 @@ class Sequence:
         end = min(start + len(k), self.rows.shape[1])
         for r, x in zip(self.rows, (k, v)):
             r[start:end] = x[:end - start]
-        since = min(self.len, start)             # tokens between len and start begin anew, too
-        self.weights[:, since:end] = 0
-        self.positions[:, since:end] = np.arange(since, end) + self.evicted
+        self.weights[:, start:end] = 0
+        self.positions[:, start:end] = np.arange(start, end) + self.evicted
         self.len = end
 
     def evict(self, keep: int, recent: int = 0, first: int = 0):

@@ -67,14 +67,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedCache c, c
     }
   }
   if (c.weights) {
-    // from the end of what was there on: tokens between it and start count as new, too
-    int since = c.lens[b];
-    since = since < 0 ? 0 : since < start ? since : start;
-    const int gone = c.evicted[b], news = start + cnt - since;
-    for (long t0 = (long)blockIdx.x * chunk; t0 < news; t0 += (long)gridDim.x * chunk) {
-      const int toks = (int)(news - t0 < chunk ? news - t0 : chunk);
+    // of the new tokens only: what lies in front of them, slots between lens and start among it, is the program's
+    const int gone = c.evicted[b];
+    for (long t0 = (long)blockIdx.x * chunk; t0 < cnt; t0 += (long)gridDim.x * chunk) {
+      const int toks = (int)(cnt - t0 < chunk ? cnt - t0 : chunk);
       for (int i = tid; i < toks * c.Hk; i += 256) {
-        const int hk = i / toks, at = since + (int)t0 + i % toks;
+        const int hk = i / toks, at = start + (int)t0 + i % toks;
         const long to = ((long)b * c.Hk + hk) * cap + at;
         c.weights[to] = 0.f;
         c.positions[to] = at + gone;
@@ -82,9 +80,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedCache c, c
     }
   }
   // The length is written when all workgroups of the sequence have read it (as the start or the
-  // count, or for the account of the tokens): by the last one, found by a ticket that wraps to 0 by
-  // itself.
-  const bool turn = start_in == c.lens || counts == c.lens || c.weights;
+  // count): by the last one, found by a ticket that wraps to 0 by itself.
+  const bool turn = start_in == c.lens || counts == c.lens;
   if (turn) __syncthreads();
   if (tid == 0) {
     const bool last = !turn ? blockIdx.x == 0

@@ -320,8 +320,10 @@ class PagedKVCache:
         counts (B,) int32: how many of the n tokens each sequence has (the rest is padding; not
         read).  start (B,) int32: append behind that many tokens in place of ``lens``; what the sequence
         held behind them is dropped, tokens between ``lens`` and start are what the pages hold (how a
-        sequence takes over a beginning that another one has).  Tokens past the capacity are
-        dropped (``lens`` stops there)."""
+        sequence takes over a beginning that another one has), and with track=True what ``weights``
+        and ``positions`` hold: the program writes those (0 and the slots' numbers for a beginning
+        that nothing was evicted from).  New tokens get weight 0 and the position slot + ``evicted``.
+        Tokens past the capacity are dropped (``lens`` stops there)."""
         what = "PagedKVCache.append"
         B, H, D = self.batch, self.kv_heads, self.head_dim
         packed = plan is not None

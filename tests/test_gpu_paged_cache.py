@@ -119,6 +119,46 @@ def test_append_counts_start_and_capacity(gpu):
     assert both.cache.lens.tolist() == [0, 320, 320, 320]
 
 
+@pytest.mark.parametrize("how", ["padded", "packed", "graph"])
+def test_append_keeps_the_account_in_front_of_start(gpu, how):
+    """What a program wrote there itself (a restored cache, a beginning of another sequence) stays, whatever lens says;
+    the new tokens' own, and nothing behind them, are written."""
+    from qvggt_amd import awq_inference_engine as E
+    both = Both(gpu, 6, 2, 64, 256, 16, F16)
+    c, n = both.cache, (3, 1, 0, 40, 10, 7)
+    lens, start, gone = [0, 5, 100, 0, 200, 256], [200, 30, 90, 64, 250, 300], [0, 7, 1000, 3, 0, 9]
+    given = torch.rand(c.weights.shape, generator=both.g, device=gpu)
+    pos = torch.randint(0, 1 << 20, c.positions.shape, generator=both.g, device=gpu, dtype=torch.int32)
+    k, v = both.kv(sum(n)) if how == "packed" else both.kv(6, 40)
+    plan = E.packed_plan(n, 2, 2, 64, device=gpu) if how == "packed" else None
+    counts, begin = None if plan else _i32(gpu, n), _i32(gpu, start)
+
+    def put():
+        c.lens.copy_(_i32(gpu, lens))
+        c.evicted.copy_(_i32(gpu, gone))
+        c.weights.copy_(given)
+        c.positions.copy_(pos)
+
+    call = lambda: c.append(k, v, counts=counts, start=begin, plan=plan)
+    if how == "graph":
+        graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=s):
+            call()
+        call = graph.replay
+    for _ in range(3):
+        put()
+        call()
+        torch.cuda.synchronize()
+        want_w, want_p = given.clone(), pos.clone()
+        for b in range(6):
+            s, e = min(start[b], 256), min(start[b] + n[b], 256)
+            want_w[b, :, s:e] = 0
+            want_p[b, :, s:e] = torch.arange(s, e, device=gpu, dtype=torch.int32) + gone[b]
+            assert c.lens[b] == e
+        assert torch.equal(c.weights, want_w) and torch.equal(c.positions, want_p)
+
+
 @pytest.mark.parametrize("D,dtype,track", [(64, BF16, False), (128, F16, True)])
 def test_append_packed(gpu, D, dtype, track):
     """Packed tokens, of a strided buffer with rows behind them."""

@@ -42,6 +42,14 @@ def test_eviction_by_hand():
     assert s.positions[0, :3].tolist() == [0, 4, 5] and s.evicted == 5
 
 
+def test_append_writes_the_account_of_its_tokens_only():
+    s = P.Sequence(8, 1, 1)
+    s.weights[:], s.positions[:], s.evicted = 5, 70, 10
+    s.append(np.zeros((2, 1, 1)), np.zeros((2, 1, 1)), start=4)              # len is 0
+    assert s.len == 6 and s.weights[0].tolist() == [5, 5, 5, 5, 0, 0, 5, 5]
+    assert s.positions[0].tolist() == [70, 70, 70, 70, 14, 15, 70, 70]
+
+
 @pytest.mark.parametrize("lens,H,Hk,frame", [((5, 0, 300, 129), 4, 2, 1), ((1000,), 8, 1, 64), ((64, 65), 2, 2, None), ((), 1, 1, 1), ((0,), 1, 1, 3),
                                              ((1374 * 3, 1374), 16, 16, 1374)])
 def test_packed_plan_covers_every_row_once(lens, H, Hk, frame):
