@@ -334,7 +334,8 @@ __device__ __forceinline__ void kv_softmax(f32x16 (&sc)[KB], float c, KvState<D>
     const bool need = mx > s.m + KV_TOP;
     if (__builtin_amdgcn_ballot_w64(need)) {
       const float m_new = need ? mx - KV_LIFT : s.m;
-      const float alpha = need ? __builtin_amdgcn_exp2f(s.m - m_new) : 1.0f;   // 0 where there was none
+      // 1 where there was none: l and O are 0 then, but for infinite values that a careful walk put there already
+      const float alpha = need && s.m != -INFINITY ? __builtin_amdgcn_exp2f(s.m - m_new) : 1.0f;
       s.m = m_new;
       s.ref = m_new == -INFINITY ? 0.f : m_new;
       s.l *= alpha;

@@ -124,6 +124,31 @@ def test_packed_non_finite_reaches_only_those_that_see_it(gpu, D, dtype, Hk, fra
     assert torch.equal(out[:300][~from_(100)], clean[:300][~from_(100)]) and torch.equal(out[300:], clean[300:])
 
 
+@pytest.mark.parametrize("D,dtype,Hk", [(64, F16, 1), (64, BF16, 1), (128, F16, 1), (128, BF16, 1), (64, F16, 256), (64, BF16, 256)])
+@pytest.mark.parametrize("frame", [1, 50, None])
+def test_packed_infinities_of_the_first_tokens(gpu, D, dtype, Hk, frame):
+    """In the first tile an infinity reaches those that see it as one, too; two of unlike signs as NaN."""
+    from qvggt_amd import awq_inference_engine as E
+    lens, H = (300, 120), 2 * Hk
+    q, k, v = _qkv(gpu, 7, sum(lens), H, Hk, D, dtype, 0.25)
+    plan = E.packed_plan(lens, H, Hk, D, frame=frame, device=gpu)
+    assert plan.rows == (256 if Hk == 256 else 128)
+    clean = E.packed_attention(q, k, v, plan)
+    bad, want, inf = v.clone(), clean.clone(), float("inf")
+    i = torch.arange(300, device=gpu)
+    from_ = lambda t: ((i // frame + 1) * frame if frame else torch.full_like(i, 300)) > t
+    for t, dim, x in ((0, 0, inf), (0, 1, -inf), (40, 2, inf), (40, 3, -inf), (63, 4, inf), (64, 5, -inf), (127, 6, inf)):
+        bad[t, 0, dim] = x
+        want[:300][from_(t), :2, dim] = x
+    bad[0, 0, 7], bad[40, 0, 7] = inf, -inf
+    want[:300][from_(0), :2, 7] = inf
+    want[:300][from_(40), :2, 7] = float("nan")
+    out = E.packed_attention(q, k, bad, plan)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf())
+    ok = ~want.isnan()
+    assert torch.equal(out[ok], want[ok])
+
+
 def test_packed_long_sequence(gpu):
     """A longer one, some heads and rows of it against the definition."""
     from qvggt_amd import awq_inference_engine as E

@@ -273,6 +273,33 @@ def test_attention_non_finite(gpu, n, H, Hk, D, dtype):
     assert torch.equal(out[ok], want[ok])
 
 
+@pytest.mark.parametrize("n,H,Hk", [(1, 1, 1), (4, 4, 1), (3, 2, 2), (32, 1, 1), (60, 2, 1), (130, 1, 1)])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (64, BF16), (128, F16), (128, BF16)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("tokens", [500, 9000])
+def test_attention_infinite_values_anywhere(gpu, tokens, causal, D, dtype, n, H, Hk):
+    """An infinity that all queries see is one in its dim, in the first tile of a wave, a share or a piece as well; two
+    of unlike signs are NaN.  (9000 tokens: shares of 256 slots.)"""
+    both = Both(gpu, 1, Hk, D, tokens, 32, dtype)
+    both.append(tokens)
+    q = both.rand(1, n, H, D) / 4                            # even weights: none comes to 0 in 32 bits
+    clean = both.attend(q, causal=causal)
+    at = lambda s: (both.cache.table[0, s // 32].long(), slice(None), s % 32)
+    inf, want = float("inf"), clean.clone()
+    slots = [0, 40, 64, 127, 128, 255, tokens - n] + ([256, 300, 4096, 4100, 8191] if tokens > 500 else [])
+    for i, s in enumerate(slots):
+        both.cache.v_pages[at(s)][:, i] = inf if i % 2 else -inf
+        want[..., i] = inf if i % 2 else -inf
+    both.cache.v_pages[at(0)][:, 40], both.cache.v_pages[at(33)][:, 40] = inf, -inf
+    want[..., 40] = float("nan")
+    both.cache.v_pages[at(1)][:, 41] = float("nan")
+    want[..., 41] = float("nan")
+    out = both.cache.attention(q, causal=causal)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf())
+    ok = ~want.isnan()
+    assert torch.equal(out[ok], want[ok])
+
+
 def test_shared_pages(gpu):
     """Two sequences read the pages of one beginning."""
     both = Both(gpu, 2, 2, 64, 256, 64, F16)
