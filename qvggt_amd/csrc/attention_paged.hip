@@ -536,7 +536,8 @@ static void kv_paged_launch(const KvPagedPlan& plan, const KvSteps& p, float* we
     if (joins + receives > 0)
       hipLaunchKernelGGL((kv_paged_finish_kernel<BF16, D>), dim3(joins + receives, a.Hk, a.B), dim3(256), 0, st, p, joins, weights);
   }
-  if (a.lse) {
+  // a pool without pages: no token receives, and the kernel's lanes without a key would have no page to read
+  if (a.lse && a.pages > 0) {
     const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>((keys + 127) / 128, 1), 4096), a.Hk, a.B);
     hipLaunchKernelGGL((kv_receive_kernel<BF16, D>), grid, dim3(256), 0, st, a, weights);
   }

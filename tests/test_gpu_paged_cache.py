@@ -433,6 +433,30 @@ def test_c_entry_without_workspace(gpu, n, H, Hk, D, dtype):
             assert torch.equal(out[:, :, :H], want)
 
 
+@pytest.mark.parametrize("n,H,slots", [(1, 4, 8), (60, 2, 8), (150, 1, 200), (1, 32, 130)])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16)])
+def test_c_entry_of_a_pool_without_pages(gpu, n, H, slots, D, dtype):
+    """No page is one: queries see nothing, and nothing is received (130 slots of 65536 tokens: scores are not kept)."""
+    from qvggt_amd import _lib
+    from qvggt_amd import awq_inference_engine as E
+    page = 65536 if slots == 130 else 64
+    cap = slots * page
+    q = torch.randn(2, n, H, D, device=gpu).to(dtype)
+    table = torch.arange(2 * slots, dtype=torch.int32, device=gpu).view(2, slots)
+    lens = _i32(gpu, [cap, 77])
+    given = torch.rand(2, 1, cap, device=gpu)
+    need = _lib.load().qv_paged_attention_workspace(1, 2, n, H, 1, D, cap, cap)
+    ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+    for weights in (None, given.clone()):
+        out = torch.full_like(q, 3.0)
+        _lib.call("qv_paged_attention", q.data_ptr(), out.data_ptr(), 1 if dtype == BF16 else 0, None, None, table.data_ptr(),
+                  lens.data_ptr(), None, 1, None if weights is None else weights.data_ptr(), 2, n, H, 1, D, page, slots, 0, cap,
+                  E._i64s(*q.stride()[:3]), E._i64s(*out.stride()[:3]), D ** -0.5, ws.data_ptr(), need,
+                  torch.cuda.current_stream().cuda_stream)
+        assert not out.any()
+        assert weights is None or torch.equal(weights, given)
+
+
 def test_two_streams_read_one_cache(gpu):
     """Attention calls of two streams at once have workspaces of their own."""
     both = Both(gpu, 4, 2, 64, 3000, 64, F16)
