@@ -286,7 +286,8 @@ class PagedKVCache:
             self.positions = torch.zeros(batch, kv_heads, self.capacity, dtype=torch.int32, **kw)
             self.evicted = torch.zeros(batch, dtype=torch.int32, **kw)
         self._tickets = torch.zeros(batch * _lib.QV_PAGED_TICKETS, dtype=torch.int32, **kw)
-        self._bound = 0
+        self._bound = 0                # how long a sequence may be by now, as far as the host knows
+        self._replayed = False         # a graph appends: any number of times, and any time
         names = ("k_pages", "v_pages", "table", "lens", "_tickets") + (("weights", "positions", "evicted") if track else ())
         self._wants = {n: (t.dtype, t.shape, t.device) for n, t in ((n, getattr(self, n)) for n in names)}
 
@@ -309,7 +310,12 @@ class PagedKVCache:
         self.lens.zero_()
         if self.evicted is not None:
             self.evicted.zero_()
-        self._bound = 0
+        self._at_most(0)
+
+    def _at_most(self, n: int) -> None:
+        """No sequence is longer than n now: what is captured has not run, and a graph may append again."""
+        if not self._replayed and (self.lens.device.type == "cpu" or not _capturing()):
+            self._bound = min(self._bound, n)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None,
                start: torch.Tensor | None = None, plan=None) -> None:
@@ -351,8 +357,9 @@ class PagedKVCache:
                       _ptr(self.lens if start is None else start), _ptr(self.lens), _ptr(self._tickets), _ptr(counts),
                       _ptr(plan.cu if packed else None), _ptr(self.evicted), _ptr(self.weights), _ptr(self.positions), B, n, T,
                       H, D, self.page, self.slots, self.pages, _kv_strides(k), _kv_strides(v), _stream(dev))
-        # how long a sequence may be by now (see Int8KVCache.append); a graph may be replayed any number of times
-        own = (start is None or start.data_ptr() == self.lens.data_ptr()) and not _capturing()
+        # how long a sequence may be by now (see Int8KVCache.append)
+        self._replayed = self._replayed or _capturing()
+        own = (start is None or start.data_ptr() == self.lens.data_ptr()) and not self._replayed
         self._bound = min(self.capacity, self._bound + n) if own else self.capacity
 
     # ------------------------------------------------------------ attention
@@ -369,8 +376,9 @@ class PagedKVCache:
         included.  bfloat16 values past 2**90 may overflow the sums.  ``out`` must not overlap q.
         longest: about how many tokens the longest sequence has, for the split of the keys over the
         chip, and for nothing else: any number gives the result.  By default the tokens of the calls
-        to ``append`` so far, and the capacity in a graph, behind one, and once one had a
-        ``start``: a program that writes ``lens`` itself, or uses little of a large capacity, says it.
+        to ``append`` so far (at most ``keep`` behind an ``evict``, none behind a ``reset``), the
+        capacity once one had a ``start``, in a graph, and for good once an ``append`` was captured:
+        a program that writes ``lens`` itself, or uses little of a large capacity, says it.
         collect: add to ``weights`` what each token receives: the probabilities that the queries of its
         key head's heads give it (a cache with track=True).
         Returns (B, n, heads, head_dim)."""
@@ -426,4 +434,4 @@ class PagedKVCache:
                 _lib.call("qv_paged_evict", _ptr(self.k_pages), _ptr(self.v_pages), _ptr(self.table), _ptr(self.lens),
                           _ptr(self.evicted), _ptr(self.weights), _ptr(self.positions), self.batch, self.kv_heads, self.head_dim,
                           self.page, self.slots, self.pages, keep, recent, first, _ptr(ws), ws_bytes, _stream(dev))
-        self._bound = min(self._bound, keep)
+        self._at_most(keep)

@@ -178,6 +178,50 @@ def test_paged_length_hint(monkeypatch):
     assert keys() == c.capacity
 
 
+def test_paged_length_hint_and_graphs(monkeypatch):
+    """What is captured has not run yet, and a graph that appends may do so any time: the host then knows no length."""
+    from qvggt_amd import kv_cache as M
+    calls, capturing = [], [False]
+    monkeypatch.setattr(M, "_on_gpu", lambda *t, what: 0)
+    monkeypatch.setattr(M, "_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(M, "_stream", lambda dev: 0)
+    monkeypatch.setattr(M, "_capturing", lambda: capturing[0])
+    monkeypatch.setattr(M._lib, "call", lambda name, *args: calls.append(args))
+    q, k = torch.zeros(2, 5, 4, 64).half(), torch.zeros(2, 200, 2, 64).half()
+    c = PagedKVCache(2, 2, 64, 4000, device="meta", track=True)    # as on a GPU
+
+    def keys():
+        c.attention(q)
+        return calls[-1][18]
+
+    c.append(k, k)
+    capturing[0] = True                      # captured, not run: the tokens are all there
+    c.evict(30)
+    c.reset()
+    capturing[0] = False
+    assert keys() == 200
+    c.evict(100)
+    assert keys() == 100
+    capturing[0] = True
+    c.append(k, k)
+    c.evict(30)
+    capturing[0] = False
+    assert keys() == c.capacity
+    c.evict(30)                              # the graph may be replayed behind these
+    assert keys() == c.capacity
+    c.reset()
+    assert keys() == c.capacity
+    c.append(k, k)
+    assert keys() == c.capacity
+
+
+def test_reset_of_a_cache_on_the_host():
+    c = PagedKVCache(2, 2, 64, 100, device="cpu", track=True)
+    c.lens.fill_(3), c.evicted.fill_(4)
+    c.reset()
+    assert not c.lens.any() and not c.evicted.any()
+
+
 def test_c_entries_refuse():
     """Bad arguments end at the C entries with a message, before any device work (pointers here are never followed)."""
     lib = _lib.load()
