@@ -427,7 +427,8 @@ int64_t qv_attention_kv_workspace(int cached, int64_t B, int64_t Lq, int64_t H, 
  * (device, int32 (ntiles, 4), 16-byte aligned): the work, in the order in which it is to start:
  * each is (first token of the sequence, L, a row r, 0) and covers the rows r .. r + tile_rows - 1
  * of the sequence, row = query * (H / Hk) + head % (H / Hk); tiles that reach outside 0 .. T are
- * left out, rows of out that none covers left as they were.  tile_rows 128, or 256 (D = 64).
+ * left out, rows of out that none covers left as they were.  tile_rows 128, or 256 (D = 64);
+ * ntiles * Hk below 2^24.
  * Strides (host): token and head, in elements, as for qv_attention_cross.  No workspace.
  */
 int qv_packed_attention(const void* q, const void* k, const void* v, void* out, int dtype,

@@ -978,7 +978,8 @@ class PackedPlan(NamedTuple):
 def packed_plan(lens, heads: int, kv_heads: int, head_dim: int, frame: int | None = 1, device=None) -> PackedPlan:
     """Plan of ``packed_attention`` for sequences of ``lens`` tokens (numbers on the host, zeros
     allowed) behind one another.  Made once for a batch, used by every layer that has these heads.
-    All tokens times (heads / kv_heads)**2 must be below 2**32.
+    All tokens times (heads / kv_heads)**2 must be below 2**32, key heads times row tiles (of 128
+    or 256 rows, a sequence's last one as full as it is) below 2**24.
 
     frame: query i of a sequence sees its tokens below (i // frame + 1) * frame: 1 causal by
     token, 1374 causal by frames of 1374 tokens, None all tokens of the sequence."""
@@ -1001,6 +1002,8 @@ def packed_plan(lens, heads: int, kv_heads: int, head_dim: int, frame: int | Non
     # 128 rows; 27480 causal 1578 and 1635; but 4 x 2048, one round of 512: 55.5 and 52.5).
     rows = 256 if head_dim == 64 and int((-(-n * group // 256)).sum()) * kv_heads >= 768 else 128
     of = -(-n * group // rows)                                       # row tiles of each sequence
+    if int(of.sum()) * kv_heads >= 1 << 24:                          # a grid has under 2**32 threads
+        _fail(f"{what}: too many row tiles: {int(of.sum())} of {kv_heads} key heads")
     seq = np.repeat(np.arange(len(n)), of)
     row = (np.arange(len(seq)) - np.repeat(np.cumsum(of) - of, of)) * rows
     last = np.minimum(row + rows, n[seq] * group) - 1

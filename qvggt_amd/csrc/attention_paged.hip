@@ -556,7 +556,8 @@ extern "C" int qv_packed_attention(const void* q, const void* k, const void* v, 
   if (int rc = qv::kv_common(a, q, out, dtype, 1, T, T, H, Hk, D, q_strides ? qs : nullptr, out_strides ? os : nullptr, scale))
     return rc;
   QV_CHECK_ARG(frame >= 1, "frame must be positive (got %lld)", (long long)frame);
-  QV_CHECK_ARG(ntiles >= 0 && ntiles * Hk <= INT32_MAX, "bad number of row tiles %lld", (long long)ntiles);
+  // a grid has under 2^32 threads
+  QV_CHECK_ARG(ntiles >= 0 && ntiles <= ((1 << 24) - 1) / Hk, "bad number of row tiles %lld", (long long)ntiles);
   QV_CHECK_ARG(tile_rows == 128 || (tile_rows == 256 && D == 64), "a tile has 128 rows, or 256 of 64 dims (got %lld)",
                (long long)tile_rows);
   if (T == 0 || ntiles == 0) return QV_OK;

@@ -88,6 +88,17 @@ def test_packed_refusals():
             E.packed_attention(*args, **kw)
 
 
+def test_packed_grids_that_a_launch_refuses():
+    """Very many short sequences: a workgroup of 256 threads for each row tile and key head, under 2^32 threads in all."""
+    with pytest.raises(RuntimeError, match="row tiles"):
+        E.packed_plan((1,) * 300000, 64, 64, 64)
+    assert E.packed_plan((1,) * 262143, 64, 64, 64).tiles.shape[0] == 262143
+    lib, st, p = _lib.load(), (C.c_int64 * 2)(128, 64), 1 << 20
+    for n, Hk in ((1 << 24, 1), (1 << 18, 64), ((1 << 63) - 1, 2)):
+        assert lib.qv_packed_attention(p, p, p, p, 0, p, n, 256, 1, 50, 64, Hk, 64, st, st, st, st, 0.1, None) == -1
+        assert "row tiles" in lib.qv_last_error().decode()
+
+
 def test_paged_refusals():
     for args, kw, msg in (((2, 2, 32, 100), {}, "head_dim"), ((0, 2, 64, 100), {}, "batch"), ((2, 0, 64, 100), {}, "kv_heads"),
                           ((2, 2, 64, 0), {}, "capacity"), ((2, 2, 64, 100), dict(page=24), "page"), ((2, 2, 64, 100), dict(page=8), "page"),
