@@ -496,7 +496,8 @@ static KvPagedPlan kv_paged_plan(bool collect, int64_t B, int64_t Lq, int64_t H,
     p.lse = collect ? kv_align(B * Lq * H * 4) : 0;
     // at least the places of the chip, at most what would be cut if all sequences were as long as the
     // longest, and 2048 pieces in all (parts of up to 273 MB)
-    if (tiles > 2 * KV_PIECE && Hk <= 512) {
+    // (the join's grid, a thread for 4 dims of each row, has under 2^32 threads)
+    if (tiles > 2 * KV_PIECE && Hk <= 512 && rows * (D / 4) <= (1ll << 32) - 256) {
       const int64_t all = B * p.row_tiles * kv_plan(false, B, Lq, H, Hk, D, keys).splits;
       p.shares = (int)std::min<int64_t>(std::max<int64_t>(all, 512 / Hk), 2048 / Hk);
     }

@@ -99,6 +99,16 @@ def test_packed_grids_that_a_launch_refuses():
         assert "row tiles" in lib.qv_last_error().decode()
 
 
+def test_paged_rows_whose_join_would_not_launch_are_not_cut():
+    """The join has a thread for 4 dims of each row of a key head, under 2^32 in all: no parts from there on."""
+    need = _lib.load().qv_paged_attention_workspace
+    for rows, D in (((1 << 27) - 8, 128), ((1 << 28) - 16, 64)):
+        assert need(0, 1, rows, 1, 1, D, 100000, 100000) > 0 and need(0, 1, rows // 2, 2, 1, D, 100000, 100000) > 0
+        assert need(0, 1, rows, 2, 2, D, 100000, 100000) > 0
+    for rows, D in ((1 << 27, 128), (1 << 28, 64)):
+        assert need(0, 1, rows, 1, 1, D, 100000, 100000) == 0 and need(0, 1, rows // 2, 2, 1, D, 100000, 100000) == 0
+
+
 def test_paged_refusals():
     for args, kw, msg in (((2, 2, 32, 100), {}, "head_dim"), ((0, 2, 64, 100), {}, "batch"), ((2, 0, 64, 100), {}, "kv_heads"),
                           ((2, 2, 64, 0), {}, "capacity"), ((2, 2, 64, 100), dict(page=24), "page"), ((2, 2, 64, 100), dict(page=8), "page"),
