@@ -288,15 +288,18 @@ class PagedKVCache:
         self._tickets = torch.zeros(batch * _lib.QV_PAGED_TICKETS, dtype=torch.int32, **kw)
         self._bound = 0                # how long a sequence may be by now, as far as the host knows
         self._replayed = False         # a graph appends: any number of times, and any time
-        names = ("k_pages", "v_pages", "table", "lens", "_tickets") + (("weights", "positions", "evicted") if track else ())
-        self._wants = {n: (t.dtype, t.shape, t.device) for n, t in ((n, getattr(self, n)) for n in names)}
+        names = ("k_pages", "v_pages", "table", "lens", "_tickets", "weights", "positions", "evicted")
+        self._wants = {n: t if t is None else (t.dtype, t.shape, t.device) for n, t in ((n, getattr(self, n)) for n in names)}
 
     _per_sequence = Int8KVCache._per_sequence
 
     def __setattr__(self, name: str, value) -> None:
         """The cache's tensors can be replaced by ones of the same type and shape on the same GPU (the
-        kernels rely on that, and no call checks it again)."""
-        want = self.__dict__.get("_wants", {}).get(name)
+        kernels rely on that, and no call checks it again); those of track=True only where it was said."""
+        wants = self.__dict__.get("_wants", {})
+        want = wants.get(name)
+        if want is None and name in wants and value is not None:
+            _fail(f"PagedKVCache: {name} belongs to a cache with track=True")
         if want is not None:
             dtype, shape, device = want
             if (not isinstance(value, torch.Tensor) or value.dtype != dtype or value.shape != shape

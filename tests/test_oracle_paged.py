@@ -163,6 +163,18 @@ def test_paged_tensors_are_replaced_by_like_ones_only():
     assert c.table is new
 
 
+def test_account_of_a_cache_that_keeps_none():
+    """Nothing would check a tensor that is put there, and the kernels would take its pointer."""
+    c = PagedKVCache(2, 2, 64, 100, device="cpu")
+    for name in ("weights", "positions", "evicted"):
+        with pytest.raises(RuntimeError, match=f"{name} belongs to a cache with track=True"):
+            setattr(c, name, torch.zeros(3))
+        assert getattr(c, name) is None
+        setattr(c, name, None)
+    with pytest.raises(RuntimeError, match="track"):
+        c.attention(torch.zeros(2, 1, 4, 64).half(), collect=True)
+
+
 def test_paged_length_hint(monkeypatch):
     """How many keys the attention's plan is laid out for.  No kernel runs here."""
     from qvggt_amd import kv_cache as M
