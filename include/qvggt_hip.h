@@ -489,7 +489,8 @@ int64_t qv_paged_attention_workspace(int collect, int64_t B, int64_t Lq, int64_t
  * those of the largest weights, the lower slot first where they are equal, NaN last: keep in
  * all.  The slots below keep that become free take, in order, the tokens kept behind keep (row,
  * weight, position); lens[b] becomes keep, evicted[b] grows by what went.  Slots behind keep are
- * left as they were.  Slots below lens need pages, which no other sequence may use.
+ * left as they were.  Slots below lens need pages, those of slots below keep no other sequence may
+ * use.  weights and positions are 16-byte aligned.
  */
 int qv_paged_evict(void* k_pages, void* v_pages, const int32_t* table, int32_t* lens,
                    int32_t* evicted, float* weights, int32_t* positions, int64_t B,

@@ -463,6 +463,8 @@ extern "C" int qv_paged_evict(void* k_pages, void* v_pages, const int32_t* table
   if (B == 0 || cap <= keep) return QV_OK;
   QV_CHECK_ARG(lens && evicted && weights && positions && table && (pages == 0 || (k_pages && v_pages)), "null pointer argument");
   QV_CHECK_ARG((uintptr_t)k_pages % 16 == 0 && (uintptr_t)v_pages % 16 == 0, "pages must be 16-byte aligned");
+  QV_CHECK_ARG((uintptr_t)weights % 16 == 0 && (uintptr_t)positions % 16 == 0,
+               "weights and positions must be 16-byte aligned");        // read four at a time
   const int64_t need = qv_paged_evict_workspace(B, Hk, cap, keep), most = std::min(keep, cap - keep);
   QV_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need, "evict takes %lld bytes of workspace",
                (long long)need);

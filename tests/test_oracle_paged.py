@@ -109,6 +109,14 @@ def test_paged_rows_whose_join_would_not_launch_are_not_cut():
         assert need(0, 1, rows, 1, 1, D, 100000, 100000) == 0 and need(0, 1, rows // 2, 2, 1, D, 100000, 100000) == 0
 
 
+def test_evict_refuses_an_account_off_16_bytes():
+    """It is read four tokens at a time."""
+    lib, p = _lib.load(), 1 << 20
+    for w, pos in ((p + 4, p), (p, p + 8)):
+        assert lib.qv_paged_evict(p, p, p, p, p, w, pos, 2, 2, 64, 16, 4, 9, 30, 3, 2, p, 1 << 20, None) == -1
+        assert "aligned" in lib.qv_last_error().decode()
+
+
 def test_paged_refusals():
     for args, kw, msg in (((2, 2, 32, 100), {}, "head_dim"), ((0, 2, 64, 100), {}, "batch"), ((2, 0, 64, 100), {}, "kv_heads"),
                           ((2, 2, 64, 0), {}, "capacity"), ((2, 2, 64, 100), dict(page=24), "page"), ((2, 2, 64, 100), dict(page=8), "page"),
