@@ -223,8 +223,8 @@ def prepare(case, seed):
                          device=st["table"].device)
     for name in ("k_pages", "v_pages", "table"):
         getattr(cache, name).copy_(st.pop(name))
-    if case["kind"] != "evict":                         # what the cache holds already
-        cache.lens.copy_(st["lens" if case["kind"] == "paged" else "start"])
+    if case["kind"] == "paged":
+        cache.lens.copy_(st["lens"])
     st["cache"] = cache
     return st
 
@@ -243,11 +243,10 @@ def run(st):
             state = (cache.positions, cache.weights) if case["track"] else ()
             return cache.k_pages, cache.v_pages, cache.lens, *state
         if kind == "paged":
-            longest = case["past"] + case["queries"]    # this program, not append, filled the cache
             if not case["collect"]:
-                return cache.attention(st["q"], causal=True, longest=longest)
+                return cache.attention(st["q"], causal=True)
             cache.weights.copy_(st["weights"])          # so that a pass adds to the same
-            return cache.attention(st["q"], causal=True, longest=longest, collect=True), cache.weights
+            return cache.attention(st["q"], causal=True, collect=True), cache.weights
         for name in ("weights", "positions", "lens", "evicted"):    # so that a pass meets the same
             getattr(cache, name).copy_(st[name])
         cache.evict(case["keep"], recent=case["recent"], first=case["first"])
