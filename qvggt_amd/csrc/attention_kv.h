@@ -291,7 +291,8 @@ __device__ __forceinline__ void kv_mask(f32x16 (&sc)[KB], uint64_t seen, int h) 
 // slot(i) is called before each of the KB * 4 groups of four, kept apart by fences
 // if FENCE (left to itself the compiler draws all LDS reads and MFMAs to the front
 // and runs out of registers).  SUM32: l sums the probabilities themselves, not what the
-// second product takes of them (what a key receives is their quotient by it).
+// second product takes of them (what a key receives is their quotient by it; over pages always, so
+// that outputs are the same bits whether what keys receive is added up or not).
 template <bool BF, int D, int KB, bool FENCE, bool SUM32, class Slot>
 __device__ __forceinline__ void kv_softmax(f32x16 (&sc)[KB], float c, KvState<D>& s, uint4 (&pf)[2 * KB], Slot&& slot) {
   constexpr int W = 8 * KB;
@@ -610,7 +611,7 @@ __device__ __forceinline__ void kv_work(const KvAttn& a, int i, int& rt, int& ti
   }
 }
 
-// A length of at least all work over the shares, or of all 2^31 slots.
+// A length of at least all work over the shares; 2^26 tiles are more than any sequence has (2^29 slots).
 __device__ __forceinline__ int kv_least(const KvAttn& a, long total) {
   const long l = (total + a.shares - 1) / a.shares;
   return l < KV_PIECE ? KV_PIECE : l > 1 << 26 ? 1 << 26 : (int)l;
@@ -854,8 +855,8 @@ struct KvTiles {
 // each CU: 1007 and 918 TF/s (a large fp16 matrix product of the library: 1170), 2.1 and 2.3
 // us a tile (one workgroup alone 1.24 and 1.55); there a wave issues in 38 and 41 % of its
 // cycles, is ready but held in 40 and 38 %, and the matrix pipe is busy in 47 and 38 %.
-// Packed: 16000 tokens of 32 / 8 heads of 128, bf16, causal 1900 us (1104 TF/s); 6 sequences of up to
-// 2900 tokens of 16 / 4 heads 93 us (810 TF/s), where 1088 workgroups of 16 tiles on average spend some 3
+// Packed: 16000 tokens of 32 / 8 heads of 128, bf16, causal 1915 us (1095 TF/s); 6 sequences of up to
+// 2900 tokens of 16 / 4 heads 97 us (784 TF/s), where 1088 workgroups of 16 tiles on average spend some 3
 // tiles' time each before and behind them.
 // 64 rows a wave would halve the LDS reads, but at D = 128 O and the queries leave no
 // registers for it: with O in accumulation registers 1374 queries of 16 heads took 112 us
@@ -1148,7 +1149,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // scale: 177).  8192 queries of 16 heads over 10992 keys, two workgroups on each CU: 940 and
 // 854 TF/s, 2.24 and 2.47 us a tile (one alone 1.36 and 1.54); a wave issues in 47 and 45 %
 // of its cycles, is ready but held in 38 and 35 %, the matrix pipe is busy in 43 and 37 %.
-// Packed: 27480 tokens of 16 heads by frames of 1374 1695 us (958 TF/s).
+// Packed: 27480 tokens of 16 heads by frames of 1374 1716 us (946 TF/s).
 // 1374 queries of 16 heads over 10992 keys: 92 us and 7 of join under a trace (86 to 90 in
 // all without); over a cache of 43968 tokens 352 and 7 (311 to 323 in all without).
 template <int SRC, bool BF16>

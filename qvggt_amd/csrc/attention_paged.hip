@@ -366,11 +366,13 @@ __global__ __launch_bounds__(256) void kv_paged_join_kernel(const KvAttn a) {
 // The scores once more, transposed: a wave keeps 32 keys of one key head in registers (a key to a lane),
 // and blocks of 64 rows, shared by the workgroup's waves, come by in LDS, the next one on its way to
 // registers meanwhile; no exponential leaves its lane before the end.  The table, the first queries and
-// their sums are asked for before the length that decides whether they are needed.  The exponentials
-// bound it (a fused multiply-add, an exponential and an addition for each score, products beside them):
-// 1374 queries of 16 heads of 64 over 31374 slots 172 us, 4.0e12 scores a second; 33 of 16 of 128 over 9033 8.6, 2 for
-// each block.  Each wave with queries of its own from memory took 377 and 15; 64 keys to a wave 162 and
-// 11.6 (fewer reads of LDS, half as many waves), 8 x 300 queries of 8 heads of 128 over up to 2300 slots 18.6 and 21.4.
+// their sums are asked for before the length that decides whether they are needed.  Vector issue
+// bounds long ones: 1374 queries of 16 heads of 64 over 31374 slots 162 us, 4.3e12 scores a second, vector
+// instructions in 93 % of the cycles, of which 54 % are a score's fused multiply-add, exponential (two
+// slots) and addition, the rest the next block's addresses, its way through registers to LDS, and masks.  Short
+// ones wait (8 x 300 queries of 8 heads of 128 over up to 2300 slots: 47 %, 17.9 us); 33 of 16 of 128 over
+// 9033 8.6, 2 for each block.  Each wave with queries of its own from memory took 377 for the long one and 15 for
+// the 33; 64 keys to a wave (fewer reads of LDS, half as many waves) 6 % less, 11.6, and 21.4 for the 8 x 300.
 constexpr int KV_RECEIVE = 64;     // rows of a block
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void kv_receive_kernel(const KvAttn a, float* weights) {

@@ -332,6 +332,7 @@ class PagedKVCache:
         sequence takes over a beginning that another one has), and with track=True what ``weights``
         and ``positions`` hold: the program writes those (0 and the slots' numbers for a beginning
         that nothing was evicted from).  New tokens get weight 0 and the position slot + ``evicted``.
+        Behind an ``evict`` slots are in no order: a start among those that it left drops any tokens.
         Tokens past the capacity are dropped (``lens`` stops there)."""
         what = "PagedKVCache.append"
         B, H, D = self.batch, self.kv_heads, self.head_dim
@@ -383,7 +384,9 @@ class PagedKVCache:
         capacity once one had a ``start``, in a graph, and for good once an ``append`` was captured:
         a program that writes ``lens`` itself, or uses little of a large capacity, says it.
         collect: add to ``weights`` what each token receives: the probabilities that the queries of its
-        key head's heads give it (a cache with track=True).
+        key head's heads give it (a cache with track=True).  Up to 32 rows (queries times heads of a key
+        head) the call's workspace has their scores over the whole capacity, B * n * heads * capacity *
+        4 bytes, where these are at most 1 GiB.
         Returns (B, n, heads, head_dim)."""
         what = "PagedKVCache.attention"
         dt, scale = _kv_query(q, self.kv_heads, out, scale, what)
